@@ -7,6 +7,8 @@ plain torch, or, where `own` is set, through this package's entry points.
 """
 
 import math
+import pathlib
+import sys
 
 import numpy as np
 import torch
@@ -233,6 +235,9 @@ def run(state):
 
 
 def _run_own(s):
+    package = str(pathlib.Path(__file__).resolve().parent.parent / "iree-adreno-genai-tuner_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     from q4llm import ops
     from q4llm.rope import Rope
     c = s["case"]
