@@ -15,7 +15,7 @@
  *   scales  [N, K/group] fp16 (bit patterns passed as uint16_t);
  *   KV caches [max_ctx, n_kv, head_dim] fp16, position-first, written in place (llama_q4.py:222-223).
  *
- * dtype codes: Q4_F32 = 0, Q4_F16 = 1.
+ * dtype codes: Q4_F32 = 0, Q4_F16 = 1; the operators over a paged cache also take Q4_BF16 = 2.
  */
 #ifndef Q4LLM_H
 #define Q4LLM_H
@@ -39,7 +39,7 @@ enum {
   Q4_ERR_HIP = -100       /* a HIP runtime call failed; q4llm_last_hip_error() has the code */
 };
 
-enum { Q4_F32 = 0, Q4_F16 = 1 };
+enum { Q4_F32 = 0, Q4_F16 = 1, Q4_BF16 = 2 };
 
 /* prologue codes of q4_gemv_fused / q4_gemv_epilogue */
 enum { Q4_PRO_NONE = 0, Q4_PRO_RMSNORM = 1, Q4_PRO_SWIGLU = 2 };
@@ -289,6 +289,100 @@ int q4_embed_lookup(const int32_t* qweight, const uint16_t* scales, const int32_
 int argmax_workspace_bytes(int64_t V, size_t* bytes);
 int argmax_f32(const float* logits, int64_t V, int32_t* out, void* workspace, size_t workspace_bytes,
                void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Batched serving over a paged KV cache (no counterpart in the reference, which steps one sequence
+ * over a dense cache): rotary positions, the write of new keys and values, attention with a prefix
+ * that the batch shares, and the check of drafted tokens. Every length, position and page is read
+ * on the device, so a captured call serves later steps with the same sizes.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Which dims of the rotated part of a head form a pair: (i, i + rot_dim / 2) or (2i, 2i + 1). */
+enum { Q4_ROPE_HALF = 0, Q4_ROPE_INTERLEAVED = 1 };
+
+/* Rotary positions: dims 0 .. rot_dim - 1 of a head are rotated, the rest stay. Pair i (a, b) at position
+ * p becomes (a c - b s, b c + a s) with c = mscale cos(p inv_freq[i]), s = mscale sin(p inv_freq[i]); the
+ * angle is formed and reduced in 64 bits. inv_freq: device fp32 [rot_dim / 2]; long-context scalings
+ * are in inv_freq and mscale. */
+typedef struct q4_rope {
+  const float* inv_freq;
+  int rot_dim;
+  int layout;
+  float mscale;
+} q4_rope;
+
+/* y = x rotated at positions[t] (device int32, any sign), or with `inverse` rotated back (the transpose: the
+ * gradient of x from that of y). x, y: T x heads x head_dim of dtype (F32, F16, BF16), rows and heads
+ * *_row and *_head elements apart (>= 0), the dims of a head next to each other. y may be x itself (same
+ * strides); other overlaps are not allowed. Arithmetic in fp32, one rounding. head_dim even and <= 1024,
+ * rot_dim even and <= head_dim, T * heads < 2^31. T == 0 does nothing. */
+int rope_rotate(const void* x, int64_t x_row, int64_t x_head, void* y, int64_t y_row, int64_t y_head, int dtype,
+                int64_t T, int heads, int head_dim, const int32_t* positions, const q4_rope* rope, int inverse,
+                void* stream);
+
+/* A paged KV cache and the batch that one step runs on it. k_cache, v_cache: [num_pages, page_size, n_kv,
+ * head_dim] of dtype F16 or BF16, num_pages * page_size < 2^31. Key j of sequence b is row j % page_size of
+ * page page_table[b * table_stride + j / page_size] (device int32; entries outside [0, num_pages) hold no
+ * key; positions from max_pages * page_size on have no page). seq_lens: device int32 [batch], the keys of
+ * each sequence, those of this step's tokens included. The T tokens of a step lie sequence after sequence:
+ * cu_q (device int32 [batch + 1], ascending from 0) gives each sequence's first, tokens from cu_q[batch] on
+ * belong to none and their outputs are left as they were; cu_q NULL: T / batch tokens each. Token i of the n
+ * tokens of sequence b has position seq_lens[b] - n + i. */
+typedef struct q4_paged_kv {
+  void* k_cache;
+  void* v_cache;
+  const int32_t* page_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_q;
+  int64_t num_pages, table_stride;
+  int dtype, page_size, n_kv, head_dim, batch, max_pages;
+} q4_paged_kv;
+
+/* Writes the keys (rotated at their positions unless `rope` is NULL) and values of the T tokens of a step to their
+ * rows of the cache, and, with q not NULL, writes q rotated the same way to q_out (which may be q itself):
+ * the batched rope_kv_write. k, v: T x n_kv x head_dim, q, q_out: T x n_q x head_dim of `dtype`: F32 or F16 with an
+ * F16 cache, BF16 with a BF16 cache; strides as in rope_rotate. A token whose position is negative writes
+ * nothing; one whose position has no page writes no key or value (its q is rotated). Two tokens of one
+ * call must not share a row. T == 0 does nothing. */
+int paged_kv_append(const q4_paged_kv* kv, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                    int64_t v_head, int dtype, int64_t T, const q4_rope* rope, const void* q, int64_t q_row,
+                    int64_t q_head, void* q_out, int64_t qo_row, int64_t qo_head, int n_q, void* stream);
+
+/* Workspace bytes of paged_attn for T tokens, n_q heads, a batch of `batch` sequences with at most L keys, the first
+ * shared_len of them shared. */
+int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
+                               size_t* bytes);
+
+/* Causal GQA attention of the T tokens of a step (q: T x n_q x head_dim, rotated; out: [T, n_q * head_dim]) over
+ * their sequences' keys: token at position p sees keys 0 .. p below L and below its sequence's length; o =
+ * softmax(scale q . k) . v, zeros where it sees none. Keys 0 .. shared_len - 1 are taken from shared_pages
+ * (device int32 [ceil(shared_len / page_size)]) for every sequence, and page_table is read for the others
+ * only: the shared keys are read and multiplied once for the whole batch. shared_len 0: shared_pages unused.
+ * dtype (of q and out): F32 or F16 with an F16 cache, BF16 with a BF16 cache; F32 keeps fp32-level
+ * accuracy (q and the softmax weights run as two fp16 terms; |q| < 65504), the others round the
+ * weights to their own type. Sums, maxima and partial results are fp32; the result does not depend on timing. q_row and
+ * q_head: elements between rows and heads, q and the strides multiples of 16 bytes, caches and out
+ * 16-byte aligned. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or 128, 0 < L, 0 <= shared_len <= L,
+ * a finite scale, shared_len <= num_pages * page_size. Keys at or past L are not read. */
+int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, int64_t q_head, void* out, int dtype, int64_t T,
+               int n_q, int L, const int32_t* shared_pages, int shared_len, float scale, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* Speculative verification. Row b of the batch drafted tokens[b][0 .. n - 1], n = n_draft[b] (device int32,
+ * clamped to [0, K]; n_draft NULL: K), token i from the probabilities draft[b][i][V]; target[b][i][V] are the
+ * target's probabilities at the same place, i = 0 .. n. Token i is accepted when uniforms[b][i] * draft[b][i][x] <
+ * target[b][i][x]; up to the first refusal j the drafted tokens stand. The next one is the lowest index
+ * whose running sum of w exceeds uniforms[b][K] * sum(w), with w = max(target[b][j] - draft[b][j], 0) at a refusal
+ * (target[b][j] if that is zero everywhere) and w = target[b][n] when all n are accepted; at most the last index of
+ * positive w, and -1 when w is zero everywhere. draft NULL: the drafts are certain (probability 1 at the
+ * token, 0 elsewhere). Negative and NaN weights count as zero. out_tokens [B, K + 1]: the accepted tokens, the
+ * next one, then -1; n_accepted [B]. Products and sums are fp64, in a fixed order. A drafted token outside
+ * [0, V) is refused. Strides in elements; rows of V next to each other. Requires B > 0, K >= 0, 0 < V < 2^31. */
+int spec_verify_workspace_bytes(int B, int K, int64_t V, size_t* bytes);
+int spec_verify(const int32_t* tokens, int64_t tok_row, const float* draft, int64_t draft_batch, int64_t draft_row,
+                const float* target, int64_t target_batch, int64_t target_row, const float* uniforms, int64_t uni_row,
+                const int32_t* n_draft, int B, int K, int64_t V, int32_t* out_tokens, int32_t* n_accepted,
+                void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Whole-model step (the exported entry points prefill_c{C}_l{L} / decode_l{L} /

@@ -430,11 +430,6 @@ __global__ __launch_bounds__(HD) void attn_combine_kernel(const float* __restric
 // smallest one >= pos + 1) issue their K/V loads before `pos` arrives; the others wait for it and
 // load nothing when empty.
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
-}
-
 // Sum over the LPK (8 or 16) aligned lanes of a key: row_mirror (i <-> 15 - i), row_half_mirror
 // (i <-> 7 - i in each half row), then quad_perm xor 1 and xor 2 -- the xor masks 15, 7, 1, 2 span
 // the lane index bits, so every lane ends with the full sum.
@@ -445,30 +440,6 @@ __device__ __forceinline__ float key_sum(float v) {
   v += dpp<0xB1>(v);
   v += dpp<0x4E>(v);
   return v;
-}
-
-template <bool kMax>
-__device__ __forceinline__ float combine2(float a, float b) {
-  return kMax ? fmaxf(a, b) : a + b;
-}
-
-// Lane swaps: xor 16 by v_permlane16_swap (odd rows of one copy trade places with even rows of
-// the other), xor 32 by v_permlane32_swap (upper half of one copy with the lower half of the
-// other). The swaps are inline asm: given one value for both operands, this compiler folds the
-// builtins' two results into the first.
-// The s_nop 1 on each side covers the VALU-write -> permlane-read and the DPP-read hazards.
-template <bool kMax>
-__device__ __forceinline__ float swap_combine16(float v) {
-  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-  return combine2<kMax>(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-}
-
-template <bool kMax>
-__device__ __forceinline__ float swap_combine32(float v) {
-  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-  return combine2<kMax>(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
 template <int HD, int NK, int G>

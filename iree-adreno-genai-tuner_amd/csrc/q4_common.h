@@ -145,6 +145,35 @@ __device__ __forceinline__ float segment_sum_to_last(float v) {
   return v;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+
+template <bool kMax>
+__device__ __forceinline__ float combine2(float a, float b) {
+  return kMax ? fmaxf(a, b) : a + b;
+}
+
+// Lane swaps: xor 16 by v_permlane16_swap (odd rows of one copy trade places with even rows of
+// the other), xor 32 by v_permlane32_swap (upper half of one copy with the lower half of the
+// other). The swaps are inline asm: given one value for both operands, this compiler folds the
+// builtins' two results into the first.
+// The s_nop 1 on each side covers the VALU-write -> permlane-read and the DPP-read hazards.
+template <bool kMax>
+__device__ __forceinline__ float swap_combine16(float v) {
+  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return combine2<kMax>(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+template <bool kMax>
+__device__ __forceinline__ float swap_combine32(float v) {
+  unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return combine2<kMax>(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
 // The fp16 (hi, lo) planes a prefill projection takes as its x operand: hi = fp16(v) (round to
 // nearest even), lo = fp16(v - hi); element k of a row sits at position (k & ~7) | 2 (k & 3) |
 // ((k >> 2) & 1), i.e. each 8-element chunk in the order (0, 4, 1, 5, 2, 6, 3, 7), the k order in

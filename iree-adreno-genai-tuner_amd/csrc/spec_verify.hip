@@ -1,0 +1,266 @@
+// Verification of drafted tokens against the target's probabilities (spec_verify).
+//
+// Row b accepts its drafted tokens x_i while u_i q_i(x_i) < p_i(x_i); at the first refusal j the next token is drawn from
+// w = max(p_j - q_j, 0), after the last acceptance from w = p_n, by inversion: the lowest index whose running sum exceeds
+// r sum(w). The product of two fp32 numbers is exact in fp64 and so is nearly every difference, and sums are
+// fp64 in a fixed order, so the choice is that of the definition but within about 1e-14 of a border.
+//
+// Two launches, each one pass: the first decides j (every workgroup for itself: two dependent round trips
+// instead of a launch) and sums w over chunks of kChunk values; the second finds the chunk by a scan of the chunk
+// sums, and reads that chunk again for the index. Only one row of p and one of q is read in full, whatever the number
+// of drafts. Bound: HBM for large batches, the dependent loads for one sequence.
+#include "q4_common.h"
+
+#include <algorithm>
+
+namespace q4 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPer = 4;                           // float4s per thread and row
+constexpr int kChunk = kThreads * 4 * kPer;       // values of a row per workgroup
+
+struct VerifyArgs {
+  const int32_t* tokens;
+  const float* draft;
+  const float* target;
+  const float* uniforms;
+  const int32_t* n_draft;
+  int64_t tok_row, draft_batch, draft_row, target_batch, target_row, uni_row;
+  int K, V, chunks;
+  double2* sums;     // [B][chunks]: of w, and of p alone
+  int32_t* out;
+  int32_t* accepted;
+};
+
+// Tokens of row b that are accepted, and how many were drafted. The same in every lane.
+__device__ __forceinline__ int accepted_of(const VerifyArgs& a, int b, int* drafted) {
+  const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.K) : a.K;
+  *drafted = n;
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < n; base += 64) {
+    const int i = base + lane;
+    bool ok = false;
+    if (i < n) {
+      const int x = a.tokens[b * a.tok_row + i];
+      if (x >= 0 && x < a.V) {
+        const double u = a.uniforms[b * a.uni_row + i];
+        const double q = a.draft ? a.draft[b * a.draft_batch + i * a.draft_row + x] : 1.0f;
+        ok = u * q < static_cast<double>(a.target[b * a.target_batch + i * a.target_row + x]);
+      }
+    }
+    const uint64_t bad = ~__ballot(ok);
+    if (bad) return min(base + __builtin_ctzll(bad), n);
+  }
+  return n;
+}
+
+// The weights of one row: w = max(p - q, 0) of the refused place, p otherwise.
+struct Weights {
+  const float* p;
+  const float* q;  // null: none
+  int zero;        // index of no weight (a certain draft that was refused), -1: none
+};
+__device__ __forceinline__ Weights weights_of(const VerifyArgs& a, int b, int j, int drafted) {
+  Weights w{a.target + b * a.target_batch + j * a.target_row, nullptr, -1};
+  if (j < drafted) {
+    if (a.draft) w.q = a.draft + b * a.draft_batch + j * a.draft_row;
+    else w.zero = a.tokens[b * a.tok_row + j];
+  }
+  return w;
+}
+
+// (w, p) of the 4 values from e on (zeros past V); rows start on whole floats, not on whole vectors.
+struct alignas(4) Quad {
+  float v[4];
+};
+__device__ __forceinline__ void load4(const float* row, int e, int V, float (&v)[4]) {
+  if (e <= V - 4) {
+    const Quad q = *reinterpret_cast<const Quad*>(row + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = e < V - i ? row[e + i] : 0.0f;
+  }
+}
+__device__ __forceinline__ double weight(const Weights& w, int e, float p, float q) {
+  const double d = e == w.zero ? 0.0 : static_cast<double>(p) - static_cast<double>(q);
+  return d > 0.0 ? d : 0.0;
+}
+__device__ __forceinline__ double positive(float p) { return p > 0.0f ? static_cast<double>(p) : 0.0; }
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+__global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
+  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
+  int drafted;
+  const int j = accepted_of(a, b, &drafted);
+  const Weights w = weights_of(a, b, j, drafted);
+  float p[kPer][4], q[kPer][4] = {};
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) load4(w.p, c * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, p[k]);
+  if (w.q) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) load4(w.q, c * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, q[k]);
+  }
+  double s = 0.0, sp = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s += weight(w, c * kChunk + (k * kThreads + threadIdx.x) * 4 + i, p[k][i], q[k][i]);
+      sp += positive(p[k][i]);
+    }
+  s = wave_sum(s);
+  sp = wave_sum(sp);
+  __shared__ double2 part[kThreads / 64];
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_double2(s, sp);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double2 t = part[0];
+    for (int i = 1; i < kThreads / 64; ++i) t.x += part[i].x, t.y += part[i].y;
+    a.sums[blockIdx.x] = t;
+    if (c == 0) a.accepted[b] = j;
+  }
+}
+
+// Inclusive running sum over the workgroup's threads; *total: of all of them. `part`: one double per wave.
+__device__ __forceinline__ double block_scan(double v, double* part, double* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double o = __shfl_up(v, m, 64);
+    if (lane >= m) v += o;
+  }
+  __syncthreads();  // the last use of part is over
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i == wave) before = all;
+    all += part[i];
+  }
+  *total = all;
+  return before + v;
+}
+
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+  const int b = blockIdx.x;
+  __shared__ double part[kThreads / 64];
+  __shared__ double before_s;
+  __shared__ int first, last, first_in, last_in;
+  const int drafted = a.n_draft ? min(max(a.n_draft[b], 0), a.K) : a.K;
+  const int j = a.accepted[b];
+  const double2* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
+  if (threadIdx.x == 0) first = a.chunks, last = -1, first_in = INT32_MAX, last_in = -1;
+  // sums over all chunks
+  double sw = 0.0, sp = 0.0, t;
+  for (int i = 0; i < a.chunks; i += kThreads) {
+    const double2 s = i + static_cast<int>(threadIdx.x) < a.chunks ? sums[i + threadIdx.x] : make_double2(0.0, 0.0);
+    block_scan(s.x, part, &t);
+    sw += t;
+    block_scan(s.y, part, &t);
+    sp += t;
+  }
+  const bool plain = !(sw > 0.0);  // nothing left of p at the refused place: p itself
+  const double limit = (plain ? sp : sw) * static_cast<double>(a.uniforms[b * a.uni_row + a.K]);
+  // the first chunk whose running sum exceeds the limit, else the last one with any weight
+  double carry = 0.0;
+  for (int i = 0; i < a.chunks; i += kThreads) {
+    const int c = i + threadIdx.x;
+    const double2 s2 = c < a.chunks ? sums[c] : make_double2(0.0, 0.0);
+    const double s = plain ? s2.y : s2.x;
+    const double run = carry + block_scan(s, part, &t);
+    if (s > 0.0) {
+      if (run > limit) atomicMin(&first, c);
+      atomicMax(&last, c);
+    }
+    __syncthreads();
+    const bool found = first < a.chunks;
+    if (found ? c == first : c == last) before_s = run - s;
+    __syncthreads();
+    if (found) break;
+    carry += t;
+  }
+  const int chunk = first < a.chunks ? first : last;
+  int next = -1;
+  if (chunk >= 0) {
+    Weights w = weights_of(a, b, j, drafted);
+    if (plain) w.q = nullptr, w.zero = -1;
+    const double before = before_s;
+    float p[kPer][4], q[kPer][4] = {};
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) load4(w.p, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, p[k]);
+    if (w.q) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) load4(w.q, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, q[k]);
+    }
+    double sum = before;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int e = chunk * kChunk + (k * kThreads + threadIdx.x) * 4;
+      double v[4], s = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = weight(w, e + i, p[k][i], q[k][i]);
+        s += v[i];
+      }
+      double run = sum + (block_scan(s, part, &t) - s);
+      sum += t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        run += v[i];
+        if (v[i] > 0.0) {
+          if (run > limit) atomicMin(&first_in, e + i);
+          atomicMax(&last_in, e + i);
+        }
+      }
+    }
+    __syncthreads();
+    next = first_in != INT32_MAX ? first_in : last_in;
+  }
+  for (int i = threadIdx.x; i <= a.K; i += kThreads)
+    a.out[static_cast<int64_t>(b) * (a.K + 1) + i] = i < j ? a.tokens[b * a.tok_row + i] : i == j ? next : -1;
+}
+
+int chunks_of(int64_t V) { return static_cast<int>((V + kChunk - 1) / kChunk); }
+
+}  // namespace
+}  // namespace q4
+
+using namespace q4;
+
+extern "C" int spec_verify_workspace_bytes(int B, int K, int64_t V, size_t* bytes) {
+  if (!bytes) return Q4_ERR_NULL;
+  if (B <= 0 || K < 0 || V <= 0 || V > INT32_MAX - kChunk || static_cast<int64_t>(B) * chunks_of(V) > INT32_MAX)
+    return Q4_ERR_SHAPE;
+  *bytes = static_cast<size_t>(B) * chunks_of(V) * sizeof(double2);
+  return Q4_OK;
+}
+
+extern "C" int spec_verify(const int32_t* tokens, int64_t tok_row, const float* draft, int64_t draft_batch,
+                           int64_t draft_row, const float* target, int64_t target_batch, int64_t target_row,
+                           const float* uniforms, int64_t uni_row, const int32_t* n_draft, int B, int K, int64_t V,
+                           int32_t* out_tokens, int32_t* n_accepted, void* workspace, size_t workspace_bytes, void* stream) {
+  if ((!tokens && K > 0) || !target || !uniforms || !out_tokens || !n_accepted || !workspace) return Q4_ERR_NULL;
+  size_t need = 0;
+  if (int st = spec_verify_workspace_bytes(B, K, V, &need)) return st;
+  if (tok_row < 0 || draft_batch < 0 || draft_row < 0 || target_batch < 0 || target_row < 0 || uni_row < 0)
+    return Q4_ERR_SHAPE;
+  if (workspace_bytes < need) return Q4_ERR_WORKSPACE;
+  if (!aligned(tokens, 4) || !aligned(draft, 4) || !aligned(target, 4) || !aligned(uniforms, 4) || !aligned(n_draft, 4) ||
+      !aligned(out_tokens, 4) || !aligned(n_accepted, 4) || !aligned(workspace, 16))
+    return Q4_ERR_ALIGN;
+  VerifyArgs a{tokens, draft, target, uniforms, n_draft, tok_row, draft_batch, draft_row, target_batch, target_row, uni_row,
+               K, static_cast<int>(V), chunks_of(V), static_cast<double2*>(workspace), out_tokens, n_accepted};
+  const hipStream_t st = as_stream(stream);
+  hipLaunchKernelGGL(verify_sum_kernel, dim3(static_cast<unsigned>(B) * a.chunks), dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL(verify_pick_kernel, dim3(B), dim3(kThreads), 0, st, a);
+  return launch_status();
+}

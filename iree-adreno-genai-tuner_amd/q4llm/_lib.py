@@ -11,7 +11,7 @@ import pathlib
 PKG = pathlib.Path(__file__).resolve().parent.parent
 LIB_PATH = PKG / "lib" / "libq4llm.so"
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 Q4_OK = 0
 STATUS_NAMES = {
@@ -64,6 +64,12 @@ SIGNATURES = {
     "q4_embed_lookup": [p, p, p, p, i32, i64, i64, i32, p],
     "argmax_workspace_bytes": [i64, C.POINTER(sz)],
     "argmax_f32": [p, i64, p, p, sz, p],
+    "rope_rotate": [p, i64, i64, p, i64, i64, i32, i64, i32, i32, p, p, i32, p],
+    "paged_kv_append": [p, p, i64, i64, p, i64, i64, i32, i64, p, p, i64, i64, p, i64, i64, i32, p],
+    "paged_attn_workspace_bytes": [i64, i32, i32, i32, i32, i32, i32, C.POINTER(sz)],
+    "paged_attn": [p, p, i64, i64, p, i32, i64, i32, i32, p, i32, f32, p, sz, p],
+    "spec_verify_workspace_bytes": [i32, i32, i64, C.POINTER(sz)],
+    "spec_verify": [p, i64, p, i64, i64, p, i64, i64, p, i64, p, i32, i32, i64, p, p, p, sz, p],
     "q4llm_step_workspace_bytes": [p, i32, i32, C.POINTER(sz)],
     "q4llm_step_plan": [p, i32, i32, p],
     "q4llm_step": [p, p, i32, p, p, p, i32, p, p, p, sz, p],

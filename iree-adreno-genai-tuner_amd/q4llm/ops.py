@@ -11,7 +11,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import F16, F32, LIB, native_calls, ptr, stream_of
+from ._lib import BF16, F16, F32, LIB, native_calls, ptr, stream_of
 
 _DT = {torch.float32: F32, torch.float16: F16}
 
@@ -423,6 +423,211 @@ def q4_gemv_t16(tiles, tile_scales, x, N, K, group, norm_w=None, eps=1e-5, epilo
     LIB.call("q4_gemv_t16", ptr(tiles), ptr(tile_scales), ptr(x), pro, ptr(norm_w), eps, epilogue,
              None if rope is None else C.addressof(rope), ptr(out), ptr(residual), N, K, group, stream_of(x.device))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# Batched serving over a paged KV cache (include/q4llm.h: q4_paged_kv)
+# ------------------------------------------------------------------------------------------------
+
+_DT3 = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+# activations -> the cache types they go with
+_CACHES = {torch.float32: torch.float16, torch.float16: torch.float16, torch.bfloat16: torch.bfloat16}
+
+
+class _RopeC(C.Structure):
+    """struct q4_rope of include/q4llm.h."""
+    _fields_ = [("inv_freq", C.c_void_p), ("rot_dim", C.c_int), ("layout", C.c_int), ("mscale", C.c_float)]
+
+
+class _PagedC(C.Structure):
+    """struct q4_paged_kv of include/q4llm.h."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_cache", "v_cache", "page_table", "seq_lens", "cu_q")] + \
+               [("num_pages", C.c_int64), ("table_stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("dtype", "page_size", "n_kv", "head_dim", "batch", "max_pages")]
+
+
+def _same_device(first, *others):
+    """Raise ValueError unless every tensor is on one ROCm device; returns the device."""
+    _dev(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}: one device expected")
+    return first.device
+
+
+def _call_on(dev, name, *args):
+    """LIB.call on dev's current stream (the last argument), with dev as the current device."""
+    if dev.index == torch.cuda.current_device():
+        LIB.call(name, *args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            LIB.call(name, *args, stream_of(dev))
+
+
+def _heads(t, name, dtype, shape):
+    """Check a [tokens, heads, head_dim] operand whose dims of a head lie next to each other, rows and heads any
+    (non-negative) strides apart."""
+    _need(t, name, dtype, shape, contiguous=False)
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: the dims of a head must be contiguous (stride(2) == 1)")
+
+
+def _rope_c(rope, hd):
+    _need(rope.inv_freq, "inv_freq", torch.float32, (None,))
+    if 2 * rope.inv_freq.numel() > hd:
+        raise ValueError(f"inv_freq: {rope.inv_freq.numel()} frequencies rotate {2 * rope.inv_freq.numel()} dims, the head has {hd}")
+    return _RopeC(ptr(rope.inv_freq), 2 * rope.inv_freq.numel(), 1 if rope.interleaved else 0, rope.mscale)
+
+
+def _paged_c(k_cache, v_cache, page_table, seq_lens, cu_q, dtype, tokens, n_kv=None, hd=None):
+    """Check the cache and batch of a paged call for `tokens` tokens of `dtype`; returns the C struct."""
+    if dtype not in _CACHES:
+        raise ValueError(f"dtype {dtype}, expected float32, float16 or bfloat16")
+    _need(k_cache, "k_cache", _CACHES[dtype], (None, None, n_kv, hd))
+    _need(v_cache, "v_cache", _CACHES[dtype], tuple(k_cache.shape))
+    _need(page_table, "page_table", torch.int32, (None, None), contiguous=False)
+    batch, most = page_table.shape
+    if most > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table: rows must be contiguous (stride(1) == 1)")
+    _need(seq_lens, "seq_lens", torch.int32, (batch,))
+    _need(cu_q, "cu_q", torch.int32, (batch + 1,))
+    if cu_q is None and batch and tokens % batch:
+        raise ValueError(f"{tokens} tokens are not the same number for each of {batch} sequences: pass cu_q")
+    pages, size, n_kv, hd = k_cache.shape
+    return _PagedC(ptr(k_cache), ptr(v_cache), ptr(page_table), ptr(seq_lens), ptr(cu_q), pages,
+                   page_table.stride(0) if batch > 1 else max(most, 1), _DT3[k_cache.dtype], size, n_kv, hd, batch, most)
+
+
+def rope_rotate(x, positions, rope, inverse=False, out=None):
+    """x [T, heads, hd] (fp32, fp16 or bf16, rows and heads may be strided) rotated at positions [T] (device int32) by
+    `rope` (q4llm.rope.Rope); `inverse` rotates back (the gradient). `out` may be x."""
+    if x.dim() != 3 or x.dtype not in _DT3:
+        raise ValueError(f"x: expected [T, heads, hd] of float32, float16 or bfloat16, got {tuple(x.shape)} {x.dtype}")
+    t, h, hd = x.shape
+    _heads(x, "x", x.dtype, (t, h, hd))
+    _need(positions, "positions", torch.int32, (t,))
+    r = _rope_c(rope, hd)
+    if out is not None:
+        _heads(out, "out", x.dtype, (t, h, hd))
+    dev = _same_device(x, positions, rope.inv_freq, out)
+    if out is None:
+        out = torch.empty(t, h, hd, dtype=x.dtype, device=dev)
+    if t == 0:
+        return out
+    _call_on(dev, "rope_rotate", ptr(x), x.stride(0), x.stride(1), ptr(out), out.stride(0), out.stride(1), _DT3[x.dtype], t, h,
+             hd, ptr(positions), C.byref(r), int(inverse))
+    return out
+
+
+def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_q=None, rope=None, q=None, q_out=None):
+    """Writes k, v [T, n_kv, hd] of a step's tokens to their rows of the caches [pages, page_size, n_kv, hd], k (and q
+    [T, n_q, hd], to q_out) rotated at their positions by `rope` (None: not rotated). page_table [batch, max_pages],
+    seq_lens [batch] (this step's tokens included) and cu_q [batch + 1] (None: T / batch tokens each) are device int32.
+    fp32 or fp16 with fp16 caches, bf16 with bf16 ones; operands may be strided (slices of a fused qkv row).
+    Returns q_out (None without q)."""
+    if k.dim() != 3:
+        raise ValueError(f"k: expected [T, n_kv, hd], got {tuple(k.shape)}")
+    t, n_kv, hd = k.shape
+    kv = _paged_c(k_cache, v_cache, page_table, seq_lens, cu_q, k.dtype, t, n_kv, hd)
+    _heads(k, "k", k.dtype, (t, n_kv, hd))
+    _heads(v, "v", k.dtype, (t, n_kv, hd))
+    r = None if rope is None else _rope_c(rope, hd)
+    if q is not None:
+        _heads(q, "q", k.dtype, (t, None, hd))
+    if q_out is not None:
+        if q is None:
+            raise ValueError("q_out without q")
+        _heads(q_out, "q_out", k.dtype, tuple(q.shape))
+    dev = _same_device(k, v, k_cache, v_cache, page_table, seq_lens, cu_q, None if rope is None else rope.inv_freq, q, q_out)
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if t == 0:
+        return q_out
+    qs, qo = (0, 0) if q is None else q.stride()[:2], (0, 0) if q is None else q_out.stride()[:2]
+    _call_on(dev, "paged_kv_append", C.byref(kv), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), _DT3[k.dtype],
+             t, None if r is None else C.byref(r), ptr(q), *qs, ptr(q_out), *qo, 0 if q is None else q.shape[1])
+    return q_out
+
+
+def paged_attn_workspace_bytes(T, n_q, n_kv, hd, batch, L, shared_len=0) -> int:
+    b = C.c_size_t(0)
+    LIB.call("paged_attn_workspace_bytes", T, n_q, n_kv, hd, batch, L, shared_len, C.byref(b))
+    return b.value
+
+
+def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shared_pages=None, shared_len=0, L=None,
+               workspace=None, out=None):
+    """Causal attention of q [T, n_q, hd] (a step's tokens, rotated; rows and heads may be strided) over the paged caches:
+    [T, n_q * hd] of q's type. Batch as in paged_kv_append; keys 0 .. shared_len - 1 come from shared_pages
+    (device int32) for every sequence and are read once for the batch. L: no sequence has more keys (None: as
+    many as a row of page_table holds; a lower bound gives shorter launches). The tokens past cu_q[-1] keep
+    what `out` holds."""
+    if q.dim() != 3:
+        raise ValueError(f"q: expected [T, n_q, hd], got {tuple(q.shape)}")
+    t, n_q, hd = q.shape
+    kv = _paged_c(k_cache, v_cache, page_table, seq_lens, cu_q, q.dtype, t, None, hd)
+    _heads(q, "q", q.dtype, (t, n_q, hd))
+    if shared_len < 0 or (shared_len and shared_pages is None):
+        raise ValueError(f"shared_len {shared_len} needs its pages")
+    if shared_len:
+        _need(shared_pages, "shared_pages", torch.int32, (None,))
+        if shared_pages.numel() * kv.page_size < shared_len:
+            raise ValueError(f"shared_pages: {shared_pages.numel()} pages of {kv.page_size} hold fewer than {shared_len} keys")
+    _need(workspace, "workspace", torch.uint8, None)
+    _need(out, "out", q.dtype, (t, n_q * hd))
+    dev = _same_device(q, k_cache, v_cache, page_table, seq_lens, cu_q, shared_pages if shared_len else None, workspace, out)
+    align = 16 // q.element_size()
+    if q.stride(0) % align or q.stride(1) % align or q.data_ptr() % 16:
+        q = q.contiguous()
+    if L is None:
+        L = min(max(kv.max_pages * kv.page_size, shared_len), (1 << 31) - 1)
+    need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len)
+    if workspace is None:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    if out is None:
+        out = torch.empty(t, n_q * hd, dtype=q.dtype, device=dev)
+    if t == 0:
+        return out
+    _call_on(dev, "paged_attn", C.byref(kv), ptr(q), q.stride(0), q.stride(1), ptr(out), _DT3[q.dtype], t, n_q, L,
+             ptr(shared_pages) if shared_len else None, shared_len, scale, ptr(workspace), workspace.numel())
+    return out
+
+
+def spec_verify_workspace_bytes(B, K, V) -> int:
+    b = C.c_size_t(0)
+    LIB.call("spec_verify_workspace_bytes", B, K, V, C.byref(b))
+    return b.value
+
+
+def spec_verify(tokens, draft_probs, target_probs, uniforms, n_draft=None, workspace=None):
+    """Speculative verification of tokens [B, K] (device int32) drafted from draft_probs [B, K, V] (None: certain drafts)
+    against target_probs [B, K + 1, V], with uniforms [B, K + 1] in [0, 1) (fp32) for the K acceptances and the
+    next token; n_draft [B] int32: how many each row drafted (None: K). Returns (tokens [B, K + 1] int32: the
+    accepted ones, the next one, then -1; accepted [B] int32). include/q4llm.h has the rule."""
+    if tokens.dim() != 2 or target_probs.dim() != 3:
+        raise ValueError(f"tokens {tuple(tokens.shape)}, target_probs {tuple(target_probs.shape)}: expected [B, K], [B, K + 1, V]")
+    b, k = tokens.shape
+    v = target_probs.shape[2]
+    _need(tokens, "tokens", torch.int32, (b, k), contiguous=False)
+    _need(draft_probs, "draft_probs", torch.float32, (b, k, v), contiguous=False)
+    _need(target_probs, "target_probs", torch.float32, (b, k + 1, v), contiguous=False)
+    _need(uniforms, "uniforms", torch.float32, (b, k + 1), contiguous=False)
+    _need(n_draft, "n_draft", torch.int32, (b,))
+    _need(workspace, "workspace", torch.uint8, None)
+    for x, name in ((tokens, "tokens"), (draft_probs, "draft_probs"), (target_probs, "target_probs"), (uniforms, "uniforms")):
+        if x is not None and x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError(f"{name}: rows must be contiguous (stride(-1) == 1)")
+    dev = _same_device(target_probs, tokens, draft_probs, uniforms, n_draft, workspace)
+    need = spec_verify_workspace_bytes(b, k, v)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty(b, k + 1, dtype=torch.int32, device=dev)
+    accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    ds = (0, 0) if draft_probs is None else draft_probs.stride()[:2]
+    _call_on(dev, "spec_verify", ptr(tokens), tokens.stride(0), ptr(draft_probs), *ds, ptr(target_probs), *target_probs.stride()[:2],
+             ptr(uniforms), uniforms.stride(0), ptr(n_draft), b, k, v, ptr(out), ptr(accepted), ptr(workspace),
+             workspace.numel())
+    return out, accepted
 
 
 # ------------------------------------------------------------------------------------------------

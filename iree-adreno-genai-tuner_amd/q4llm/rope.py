@@ -1,4 +1,5 @@
-"""RoPE cos/sin tables for LlamaQ4 (the tables of llama_q4.py:184-192).
+"""RoPE cos/sin tables for LlamaQ4 (the tables of llama_q4.py:184-192), and the frequencies that the
+batched operators (ops.rope_rotate, ops.paged_kv_append) form their angles from.
 
 The reference takes its tables from transformers' LlamaRotaryEmbedding. They are computed here
 without transformers, with the same fp32 tensor expressions (default RoPE and the Llama-3 frequency
@@ -8,8 +9,21 @@ rows of them.
 """
 
 import math
+from typing import NamedTuple
 
 import torch
+
+
+class Rope(NamedTuple):
+    """Rotary positions of the batched operators (q4_rope in include/q4llm.h): inv_freq [rot_dim / 2] fp32 (the first
+    rot_dim dims of a head are rotated), pairs (2i, 2i + 1) if interleaved else (i, i + rot_dim / 2), and the
+    factor on cos and sin."""
+    inv_freq: torch.Tensor
+    interleaved: bool = False
+    mscale: float = 1.0
+
+    def to(self, device):
+        return self._replace(inv_freq=self.inv_freq.to(device))
 
 
 def _rope_params(cfg: dict) -> dict:
@@ -52,3 +66,42 @@ def rope_tables(cfg: dict, max_ctx: int):
     ang = (inv[None, :, None] @ pos).transpose(1, 2)[0]  # [max_ctx, hd/2], one fp32 product each
     emb = torch.cat((ang, ang), dim=-1)
     return emb.cos() * 1.0, emb.sin() * 1.0
+
+
+def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Rope:
+    """The Rope of a model config: partial heads (partial_rotary_factor) and the scalings for long contexts
+      default, llama3   as inv_freq
+      linear            frequencies / factor (position interpolation)
+      dynamic           base grown with seq_len past the trained length (NTK-aware scaling)
+      yarn              frequencies of long wavelengths interpolated, those of short ones kept, in between a ramp over
+                        the dims from beta_fast to beta_slow turns within the trained length; cos and sin times
+                        attention_factor, or 0.1 ln(factor) + 1 (Peng et al. 2023)
+    on the host; `.to(device)` for the operators."""
+    p = _rope_params(cfg)
+    hd = cfg.get("head_dim") or cfg["hidden_size"] // cfg["num_attention_heads"]
+    d = int(hd * p.get("partial_rotary_factor", cfg.get("partial_rotary_factor", 1.0)))
+    kind = p["rope_type"]
+    if kind in ("default", "llama3"):
+        return Rope(inv_freq({**cfg, "head_dim": d}), interleaved)
+    base, factor = p["rope_theta"], p["factor"]
+    exps = torch.arange(0, d, 2, dtype=torch.int64).to(dtype=torch.float) / d
+    trained = p.get("original_max_position_embeddings") or cfg["max_position_embeddings"]
+    if kind == "linear":
+        return Rope(1.0 / (base ** exps) / factor, interleaved)
+    if kind == "dynamic":
+        n = max(seq_len or trained, trained)
+        return Rope(1.0 / ((base * ((factor * n / trained) - (factor - 1)) ** (d / (d - 2))) ** exps), interleaved)
+    if kind != "yarn":
+        raise NotImplementedError(f"rope_type {kind!r}")
+
+    def dim_of(turns):  # the dim whose wavelength makes `turns` turns within the trained length
+        return d * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    lo = max(math.floor(dim_of(p.get("beta_fast") or 32)), 0)
+    hi = min(math.ceil(dim_of(p.get("beta_slow") or 1)), d - 1)
+    ramp = ((torch.arange(d // 2, dtype=torch.float) - lo) / (hi - lo if hi != lo else 0.001)).clamp(0, 1)
+    inv = 1.0 / (base ** exps)
+    mscale = p.get("attention_factor")
+    if mscale is None:
+        mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return Rope(inv / factor * ramp + inv * (1 - ramp), interleaved, float(mscale))
