@@ -129,71 +129,101 @@ __global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
   }
 }
 
-// Inclusive running sum over the workgroup's threads; *total: of all of them. `part`: one double per wave.
-__device__ __forceinline__ double block_scan(double v, double* part, double* total) {
+// Inclusive running sums over the threads of the workgroup, of N values at once; total[k]: of all threads. `part`: N doubles
+// per wave, free on entry; the caller synchronises before it is used again.
+template <int N>
+__device__ __forceinline__ void block_scan(double (&v)[N], double (*part)[N], double (&total)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    const double o = __shfl_up(v, m, 64);
-    if (lane >= m) v += o;
-  }
-  __syncthreads();  // the last use of part is over
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  double before = 0.0, all = 0.0;
+    double o[N];
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
-    if (i == wave) before = all;
-    all += part[i];
+    for (int k = 0; k < N; ++k) o[k] = __shfl_up(v[k], m, 64);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (lane >= m) v[k] += o[k];
   }
-  *total = all;
-  return before + v;
+  if (lane == 63)
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[wave][k] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    double before = 0.0, all = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i == wave) before = all;
+      all += part[i][k];
+    }
+    total[k] = all;
+    v[k] += before;
+  }
+}
+
+// The least `lo` and the largest `hi` of the workgroup, in every thread. `part`: free on entry.
+__device__ __forceinline__ int2 block_min_max(int lo, int hi, int2* part) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    lo = min(lo, __shfl_xor(lo, m, 64));
+    hi = max(hi, __shfl_xor(hi, m, 64));
+  }
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_int2(lo, hi);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) lo = min(lo, part[i].x), hi = max(hi, part[i].y);
+  return make_int2(lo, hi);
 }
 
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const int b = blockIdx.x;
-  __shared__ double part[kThreads / 64];
-  __shared__ double before_s;
-  __shared__ int first, last, first_in, last_in;
+  __shared__ double sums_s[kThreads / 64][2], in_s[kThreads / 64][kPer], before_s;
+  __shared__ int2 mm[2][kThreads / 64];
   const int drafted = a.n_draft ? min(max(a.n_draft[b], 0), a.K) : a.K;
   const int j = a.accepted[b];
+  const double u = a.uniforms[b * a.uni_row + a.K];
   const double2* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
-  if (threadIdx.x == 0) first = a.chunks, last = -1, first_in = INT32_MAX, last_in = -1;
-  // sums over all chunks
-  double sw = 0.0, sp = 0.0, t;
-  for (int i = 0; i < a.chunks; i += kThreads) {
-    const double2 s = i + static_cast<int>(threadIdx.x) < a.chunks ? sums[i + threadIdx.x] : make_double2(0.0, 0.0);
-    block_scan(s.x, part, &t);
-    sw += t;
-    block_scan(s.y, part, &t);
-    sp += t;
+  auto load = [&](int c) { return c < a.chunks ? sums[c] : make_double2(0.0, 0.0); };
+  // the sums of all chunks; one tile of kThreads chunks (1 M values) is kept with its running sums
+  const double2 mine = load(threadIdx.x);
+  double run[2] = {mine.x, mine.y}, all[2];
+  block_scan(run, sums_s, all);
+  for (int i = kThreads; i < a.chunks; i += kThreads) {
+    const double2 s = load(i + threadIdx.x);
+    double v[2] = {s.x, s.y}, t[2];
+    __syncthreads();
+    block_scan(v, sums_s, t);
+    all[0] += t[0], all[1] += t[1];
   }
-  const bool plain = !(sw > 0.0);  // nothing left of p at the refused place: p itself
-  const double limit = (plain ? sp : sw) * static_cast<double>(a.uniforms[b * a.uni_row + a.K]);
+  const int f = all[0] > 0.0 ? 0 : 1;  // nothing left of p at the refused place: p itself
+  const double limit = all[f] * u;
   // the first chunk whose running sum exceeds the limit, else the last one with any weight
   double carry = 0.0;
+  int chunk = -1;
   for (int i = 0; i < a.chunks; i += kThreads) {
     const int c = i + threadIdx.x;
-    const double2 s2 = c < a.chunks ? sums[c] : make_double2(0.0, 0.0);
-    const double s = plain ? s2.y : s2.x;
-    const double run = carry + block_scan(s, part, &t);
-    if (s > 0.0) {
-      if (run > limit) atomicMin(&first, c);
-      atomicMax(&last, c);
+    double s = f ? mine.y : mine.x, r = run[f], t = 0.0;
+    if (a.chunks > kThreads) {  // more than one tile: again, with the sums of those before
+      const double2 s2 = load(c);
+      s = f ? s2.y : s2.x;
+      double v[1] = {s}, w[1];
+      __syncthreads();
+      block_scan(v, reinterpret_cast<double(*)[1]>(&in_s[0][0]), w);
+      r = carry + v[0];
+      t = w[0];
     }
-    __syncthreads();
-    const bool found = first < a.chunks;
-    if (found ? c == first : c == last) before_s = run - s;
+    const int2 at = block_min_max(s > 0.0 && r > limit ? c : INT32_MAX, s > 0.0 ? c : -1, mm[0]);
+    const bool found = at.x != INT32_MAX;
+    if (found) chunk = at.x;
+    else if (at.y >= 0) chunk = at.y;
+    if (c == chunk) before_s = r - s;
     __syncthreads();
     if (found) break;
     carry += t;
   }
-  const int chunk = first < a.chunks ? first : last;
   int next = -1;
   if (chunk >= 0) {
     Weights w = weights_of(a, b, j, drafted);
-    if (plain) w.q = nullptr, w.zero = -1;
-    const double before = before_s;
+    if (f) w.q = nullptr, w.zero = -1;
     float p[kPer][4], q[kPer][4] = {};
 #pragma unroll
     for (int k = 0; k < kPer; ++k) load4(w.p, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, p[k]);
@@ -201,29 +231,33 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
 #pragma unroll
       for (int k = 0; k < kPer; ++k) load4(w.q, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, q[k]);
     }
-    double sum = before;
+    double s[kPer], t[kPer];
+    auto value = [&](int k, int i) { return weight(w, chunk * kChunk + (k * kThreads + threadIdx.x) * 4 + i, p[k][i], q[k][i]); };
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) s[k] = ((value(k, 0) + value(k, 1)) + value(k, 2)) + value(k, 3);
+    double own[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) own[k] = s[k];
+    block_scan(s, in_s, t);
+    double before = before_s;
+    int lo = INT32_MAX, hi = -1;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int e = chunk * kChunk + (k * kThreads + threadIdx.x) * 4;
-      double v[4], s = 0.0;
+      double r = before + (s[k] - own[k]);
+      before += t[k];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[i] = weight(w, e + i, p[k][i], q[k][i]);
-        s += v[i];
-      }
-      double run = sum + (block_scan(s, part, &t) - s);
-      sum += t;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        run += v[i];
-        if (v[i] > 0.0) {
-          if (run > limit) atomicMin(&first_in, e + i);
-          atomicMax(&last_in, e + i);
+        const double v = value(k, i);
+        r += v;
+        const int e = chunk * kChunk + (k * kThreads + threadIdx.x) * 4 + i;
+        if (v > 0.0) {
+          if (r > limit) lo = min(lo, e);
+          hi = max(hi, e);
         }
       }
     }
-    __syncthreads();
-    next = first_in != INT32_MAX ? first_in : last_in;
+    const int2 at = block_min_max(lo, hi, mm[1]);
+    next = at.x != INT32_MAX ? at.x : at.y;
   }
   for (int i = threadIdx.x; i <= a.K; i += kThreads)
     a.out[static_cast<int64_t>(b) * (a.K + 1) + i] = i < j ? a.tokens[b * a.tok_row + i] : i == j ? next : -1;
