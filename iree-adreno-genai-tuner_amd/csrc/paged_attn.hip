@@ -17,11 +17,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kRows = 16;  // rows (token, query head of the group) of a workgroup
-constexpr int kKeys = 32;  // keys of a wave's block
+constexpr int kKeys = 32;   // keys of a wave's block (streaming form)
+constexpr int kStage = 64;  // keys of a workgroup's stage (shared form)
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <int CT>
 using vec8 = typename Num<CT>::type __attribute__((ext_vector_type(8)));
 
@@ -31,10 +33,22 @@ __device__ __forceinline__ f32x4 mfma16(vec8<Q4_F16> a, vec8<Q4_F16> b, f32x4 c)
 __device__ __forceinline__ f32x4 mfma16(vec8<Q4_BF16> a, vec8<Q4_BF16> b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x16 mfma32(vec8<Q4_F16> a, vec8<Q4_F16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(vec8<Q4_BF16> a, vec8<Q4_BF16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 // Transposing LDS read: the lanes of each 16 read a 4 x 16 block of 16-bit values (lane i: row i / 4, columns
 // 4 (i % 4) ..) and lane i receives column i.
-__device__ __forceinline__ short4v read_tr4(void* p) {
+__device__ __forceinline__ short4v read_tr4(const void* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
+}
+// The largest of three (a NaN loses); fmaxf costs an instruction per operand more, to quiet signalling NaNs.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 struct AttnArgs {
@@ -47,10 +61,21 @@ struct AttnArgs {
   const int32_t* shared_pages;
   int T, n_q, n_kv, g, L, shared_len;
   int shared_blocks, shared_splits, shared_keys;  // workgroups of the shared ranges, ranges, keys of a range
+  int shared_tile;                                // rows of a shared workgroup
   int own_splits, parts;
   float cs, sign;  // exponents are s * cs in log2 units; sign: that of the scale, taken into q
   FastDiv by_g, by_kv, by_shared, by_own;
 };
+
+// Rows (token, head of the group) of a workgroup where there are `rows` in all. Up to 32 rows are not enough to share the
+// keys among waves: each wave streams blocks of its own (paged_stream). Past them the waves share stages of keys
+// in LDS (paged_shared), 32 rows a wave: two waves for the rows and two for the keys, or four for the rows. With two
+// terms of q and P (`split`) 32 streamed rows do not fit the registers.
+__host__ __device__ __forceinline__ int tile_rows(int64_t rows, bool split) {
+  if (rows <= 16) return 16;
+  if (rows <= 32 && !split) return 32;
+  return rows <= 64 || (rows > 128 && rows <= 192) ? 64 : 128;
+}
 
 // The sequence of token t, another in each lane (batch or more: none). Every lane of the wave takes part.
 __device__ __forceinline__ int sequence_of_lane(const PagedBatch& b, int t) {
@@ -71,10 +96,15 @@ __device__ __forceinline__ int2 tokens_of(const PagedBatch& b, int seq, int T) {
   return make_int2(c0, min(max(b.cu[seq + 1], c0), T) - c0);
 }
 
+__host__ __device__ __forceinline__ int tiles_of(int64_t rows, bool split) {
+  const int h = tile_rows(rows, split);
+  return static_cast<int>((rows + h - 1) / h);
+}
+
 // The sequence and, within it, the row tile of own tile `tile` (wave-uniform); false: past the last.
-__device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, int* seq, int* in_seq) {
+__device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, bool split, int* seq, int* in_seq) {
   if (!a.b.cu) {
-    const int per = (a.b.rows * a.g + kRows - 1) / kRows;
+    const int per = tiles_of(static_cast<int64_t>(a.b.rows) * a.g, split);
     *seq = tile / per;
     *in_seq = tile - *seq * per;
     return *seq < a.b.batch;
@@ -83,7 +113,7 @@ __device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, int* seq, 
   int base = 0;
   for (int i = 0; i < a.b.batch; i += 64) {
     const int s = min(i + lane, a.b.batch - 1);
-    const int n = i + lane < a.b.batch ? (tokens_of(a.b, s, a.T).y * a.g + kRows - 1) / kRows : 0;
+    const int n = i + lane < a.b.batch ? tiles_of(static_cast<int64_t>(tokens_of(a.b, s, a.T).y) * a.g, split) : 0;
     int run = n;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -102,123 +132,178 @@ __device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, int* seq, 
   return false;
 }
 
-// V's 16-byte chunks of a row in LDS, swizzled so that the four rows of a transposing read fall in different banks.
+// Swizzles of the 16-byte chunks of a key's row in LDS: V so that the four rows of a transposing read fall in different
+// banks, K so that 16 rows at one chunk do.
 template <int HD>
 __device__ __forceinline__ int vswz(int r) {
   return HD == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
 }
+template <int HD>
+__device__ __forceinline__ int kswz(int r) {
+  return HD == 128 ? (r & 15) : ((r >> 1) & 7);
+}
 
-// Workgroup: 16 rows of one KV head against one range of keys, 32-key blocks dealt to its four waves, which keep
-// (m, l, o) of their own and join them at the end.
+// What a workgroup does: the tile of rows, the keys k0 .. k1 - 1 of its range, and where the range's result goes.
+struct Item {
+  bool shared;
+  int h, seq, row0, n_rows, tok0, part;  // rows row0 .. of the n_rows that start at token tok0
+  int k0, k1, own_end;                   // own_end: the keys of the sequence (own ranges)
+  int behind;                            // own ranges: position of a token = behind + its index in the sequence
+};
+
+// One row: its token and head, and how many keys of the range's kind it sees (0: none, or no row). Wave-uniform flow.
+struct Row {
+  int token, head, lim;
+  bool ok;
+};
+__device__ __forceinline__ Row row_of(const AttnArgs& a, const Item& it, int r) {
+  Row w;
+  w.ok = r < it.n_rows;
+  const int i = a.by_g.div(r);
+  w.token = it.tok0 + i;
+  w.head = it.h * a.g + r - i * a.g;
+  w.lim = 0;
+  if (it.shared) {
+    const int s = sequence_of_lane(a.b, w.ok ? w.token : 0);
+    if (w.ok && s < a.b.batch) {
+      const int2 tk = tokens_of(a.b, s, a.T);
+      w.ok = w.token >= tk.x && w.token < tk.x + tk.y;
+      w.lim = min(min(a.b.lens[s] - tk.y + (w.token - tk.x) + 1, a.b.keys(s)), a.shared_len);
+    } else {
+      w.ok = false;
+    }
+  } else {
+    w.lim = min(it.behind + i + 1, it.own_end);
+  }
+  if (!w.ok) w.lim = 0;
+  return w;
+}
+
+// Eight consecutive values of a row of q as the B operand (with fp32: two fp16 terms), times the scale's sign; zeros where
+// there is no row.
+template <int QT, int CT>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const Row& w, int d, vec8<CT>* hi_out, vec8<CT>* lo_out) {
+  typedef typename Num<QT>::type Q;
+  typedef vec8<CT> C8;
+  const Q* p = static_cast<const Q*>(a.q) + w.token * a.qr + w.head * a.qh + d;
+  if constexpr (QT == Q4_F32) {
+    f32x4 x = {}, y = {};
+    if (w.ok) {
+      x = *reinterpret_cast<const f32x4*>(p);
+      y = *reinterpret_cast<const f32x4*>(p + 4);
+    }
+    const float neg1 = minus_one();
+    uint32_t hi[4], lo[4];
+    split_f16_pair(a.sign * x.x, a.sign * x.y, neg1, hi[0], lo[0]);
+    split_f16_pair(a.sign * x.z, a.sign * x.w, neg1, hi[1], lo[1]);
+    split_f16_pair(a.sign * y.x, a.sign * y.y, neg1, hi[2], lo[2]);
+    split_f16_pair(a.sign * y.z, a.sign * y.w, neg1, hi[3], lo[3]);
+    *hi_out = __builtin_bit_cast(C8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    *lo_out = __builtin_bit_cast(C8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+  } else {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (w.ok) x = *reinterpret_cast<const uint4*>(p);
+    const uint32_t flip = a.sign < 0.0f ? 0x80008000u : 0u, keep = a.sign == 0.0f ? 0u : 0xffffffffu;
+    x.x = (x.x ^ flip) & keep, x.y = (x.y ^ flip) & keep, x.z = (x.z ^ flip) & keep, x.w = (x.w ^ flip) & keep;
+    *hi_out = __builtin_bit_cast(C8, x);
+  }
+}
+
+// Eight softmax weights as the B operand of P V: two fp16 terms with fp32 activations, else rounded to the cache's type; the
+// sum is that of what is multiplied, so that a row's weights add to 1.
+template <int QT, int CT>
+__device__ __forceinline__ void weights8(const float (&p)[8], float neg1, vec8<CT>* hi_out, vec8<CT>* lo_out, float* sum) {
+  typedef vec8<CT> C8;
+  if constexpr (QT == Q4_F32) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_f16_pair(p[2 * i], p[2 * i + 1], neg1, hi[i], lo[i]);
+    *hi_out = __builtin_bit_cast(C8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    *lo_out = __builtin_bit_cast(C8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *sum += p[i];
+  } else {
+    C8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      r[i] = static_cast<typename Num<CT>::type>(p[i]);
+      *sum += static_cast<float>(r[i]);
+    }
+    *hi_out = r;
+  }
+}
+
+// N consecutive values of a range's o (or, with one range, of the result) of a row.
+template <int QT, int HD, int N>
+__device__ __forceinline__ void store_o(const AttnArgs& a, const Row& w, int part, int d, const float (&v)[N], float m,
+                                        float l) {
+  typedef typename Num<QT>::type Q;
+  const int64_t row = static_cast<int64_t>(w.token) * a.n_q + w.head;
+  if (a.parts == 1) {
+    const float inv = l > 0.0f ? 1.0f / l : l;  // no keys: zeros; NaN stays
+    struct alignas(N * sizeof(Q) < 16 ? N * sizeof(Q) : 16) V {
+      Q v[N];
+    } y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y.v[i] = static_cast<Q>(v[i] * inv);
+    *reinterpret_cast<V*>(static_cast<Q*>(a.out) + row * HD + d) = y;
+  } else {
+    const int64_t i = row * a.parts + part;
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      *reinterpret_cast<f32x4*>(a.o + i * HD + d + j) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+    if (d == 0) *reinterpret_cast<float2*>(a.ml + 2 * i) = make_float2(m, l);
+  }
+}
+
+constexpr int lds_bytes(int HD) { return std::max(4 * kStage * HD * 2, kWaves * 32 * (HD + 4) * 4); }
+
+// Streaming form: 16 RT rows of one KV head, 32-key blocks dealt to the four waves, which keep (m, l, o) of their own and
+// join them at the end. What bounds it is the latency and bandwidth of the key loads.
 //
 // Per block and wave: S^T = K Q^T (16x16x32 MFMA; K straight from memory to the A operand: lane r16 + 16 quad holds key
 // r16, dims 32 t + 8 quad ..), softmax per column (a lane holds 8 keys of one row, the other quads the rest), O^T +=
 // V^T P^T. The S^T accumulators are the P^T operand as they stand: k slots 8 quad + j carry keys 4 quad + j and 16 +
 // 4 quad + j - 4, and V^T comes from a row-major copy of the block in LDS in the same order by transposing reads.
 // The loads of the next block are issued when this one's registers are free, and cross its softmax and PV.
-template <int QT, int CT, int HD>
-__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
-  typedef typename Num<QT>::type Q;
-  typedef typename Num<CT>::type C;
+template <int QT, int CT, int HD, int RT>
+__device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, unsigned char* lds, float2 (*wml)[64]) {
   typedef vec8<CT> C8;
-  constexpr bool kSplit = QT == Q4_F32;     // q and P as two fp16 terms
+  constexpr bool kSplit = QT == Q4_F32;      // q and P as two fp16 terms
   constexpr int KS = HD / 32, OT = HD / 16;  // MFMA steps over the dims; 16-dim output tiles
   constexpr int kRowB = HD * 2;
   constexpr int kCpr = HD / 8;               // 16-byte chunks per row
   constexpr int kVld = kKeys * kCpr / 64;    // V loads per lane
   constexpr int kRpi = 64 / kCpr;            // rows per load instruction
   constexpr int kPitch = HD + 4;             // floats per row of the join buffer
-  constexpr int kBuf = std::max(kKeys * kRowB, kRows * kPitch * 4);
-  __shared__ __attribute__((aligned(16))) unsigned char buf[kWaves][kBuf];
-  __shared__ float2 wml[kWaves][kRows];
+  constexpr int kBuf = 16 * RT * kPitch * 4; // of a wave: a V block, then its rows of o
+  static_assert(kBuf >= kKeys * kRowB && kWaves * kBuf <= lds_bytes(HD), "LDS of a wave");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, quad = lane >> 4;
+  unsigned char* vb = lds + wave * kBuf;
 
-  // What this workgroup does: rows and keys.
-  int idx = blockIdx.x;
-  const bool shared = idx < a.shared_blocks;
-  if (!shared) idx -= a.shared_blocks;
-  const int hs = a.by_kv.div(idx), h = idx - hs * a.n_kv;
-  const FastDiv by_split = shared ? a.by_shared : a.by_own;
-  int tile = by_split.div(hs);
-  const int split = hs - tile * static_cast<int>(by_split.d);
-  int seq = 0, token, lim = 0, row_g, k0, k1;
-  bool row_ok;
-  if (shared) {
-    const int r = tile * kRows + r16;
-    token = a.by_g.div(r);
-    row_g = r - token * a.g;
-    row_ok = token < a.T;
-    const int s = sequence_of_lane(a.b, row_ok ? token : 0);
-    row_ok = row_ok && s < a.b.batch;
-    if (row_ok) {
-      const int2 tk = tokens_of(a.b, s, a.T);
-      row_ok = token >= tk.x && token < tk.x + tk.y;
-      lim = min(min(a.b.lens[s] - tk.y + (token - tk.x) + 1, a.b.keys(s)), a.shared_len);
-    }
-    k0 = split * a.shared_keys;
-    k1 = min(k0 + a.shared_keys, a.shared_len);
-  } else {
-    if (!own_tile(a, tile, &seq, &tile)) return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    const int2 tk = tokens_of(a.b, seq, a.T);
-    const int r = tile * kRows + r16;
-    const int i = a.by_g.div(r);
-    row_g = r - i * a.g;
-    token = tk.x + i;
-    row_ok = i < tk.y;
-    const int end = min(a.b.keys(seq), a.L);
-    lim = min(a.b.lens[seq] - tk.y + i + 1, end);
-    const int n = max(end - a.shared_len, 0);
-    const int per = ((n + a.own_splits - 1) / a.own_splits + kKeys - 1) / kKeys * kKeys;
-    k0 = a.shared_len + min(split * per, n);
-    k1 = min(k0 + per, end);
+  Row w[RT];
+  C8 qv[RT][KS], ql[RT][kSplit ? KS : 1];
+  int most = 0, least = INT32_MAX;  // the keys any row sees; those that every row sees
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    w[x] = row_of(a, it, it.row0 + 16 * x + r16);
+    most = max(most, w[x].lim);
+    if (w[x].ok) least = min(least, w[x].lim);
+#pragma unroll
+    for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w[x], 32 * t + 8 * quad, &qv[x][t], &ql[x][kSplit ? t : 0]);
   }
-  if (!row_ok) lim = 0;
-  // the last key any row sees, and the first block that some row does not see whole
-  int most = lim, least = row_ok ? lim : INT32_MAX;
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) {
     most = max(most, __shfl_xor(most, m, 64));
     least = min(least, __shfl_xor(least, m, 64));
   }
-  k1 = __builtin_amdgcn_readfirstlane(min(k1, most));
+  const int k1 = __builtin_amdgcn_readfirstlane(min(it.k1, most));
   least = __builtin_amdgcn_readfirstlane(least);
-  const int head = h * a.g + row_g;
-
-  // Q^T operand: column r16, dims 32 t + 8 quad ..
-  C8 qv[KS], ql[kSplit ? KS : 1];
-  {
-    const Q* qp = static_cast<const Q*>(a.q) + token * a.qr + head * a.qh + 8 * quad;
-    const float neg1 = minus_one();
-#pragma unroll
-    for (int t = 0; t < KS; ++t) {
-      if constexpr (kSplit) {
-        f32x4 x = {}, y = {};
-        if (row_ok) {
-          x = *reinterpret_cast<const f32x4*>(qp + 32 * t);
-          y = *reinterpret_cast<const f32x4*>(qp + 32 * t + 4);
-        }
-        uint32_t hi[4], lo[4];
-        split_f16_pair(a.sign * x.x, a.sign * x.y, neg1, hi[0], lo[0]);
-        split_f16_pair(a.sign * x.z, a.sign * x.w, neg1, hi[1], lo[1]);
-        split_f16_pair(a.sign * y.x, a.sign * y.y, neg1, hi[2], lo[2]);
-        split_f16_pair(a.sign * y.z, a.sign * y.w, neg1, hi[3], lo[3]);
-        qv[t] = __builtin_bit_cast(C8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-        ql[t] = __builtin_bit_cast(C8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-      } else {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row_ok) x = *reinterpret_cast<const uint4*>(qp + 32 * t);
-        const uint32_t flip = a.sign < 0.0f ? 0x80008000u : 0u, keep = a.sign == 0.0f ? 0u : 0xffffffffu;
-        x.x = (x.x ^ flip) & keep, x.y = (x.y ^ flip) & keep, x.z = (x.z ^ flip) & keep, x.w = (x.w ^ flip) & keep;
-        qv[t] = __builtin_bit_cast(C8, x);
-      }
-    }
-  }
 
   // Keys of a block: lane l (and l + 32) looks up key kb + l.
-  const int32_t* pages = shared ? a.shared_pages : a.b.table + seq * a.b.stride;
+  const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
   const int kl = lane & 31;
   auto page_entry = [&](int kb) {
     const int j = kb + kl;
@@ -229,33 +314,36 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     return j < k1 ? a.b.slot(entry, j - a.b.by_page.div(j) * a.b.page_size) : -1;
   };
   const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
-  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + h * kRowB + 16 * quad;
-  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + h * kRowB + 16 * (lane % kCpr);
-  uint4 kr[2][KS], vr[kVld];
+  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + 16 * quad;
+  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + 16 * (lane % kCpr);
+  u32x4 kr[2][KS], vr[kVld];
   auto load = [&](int slot) {  // keys without a row read row 0: their scores are masked, their values cleared
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int s = __shfl(slot, 16 * u + r16, 64);
       const unsigned char* p = kbase + max(s, 0) * pitch;
 #pragma unroll
-      for (int t = 0; t < KS; ++t) kr[u][t] = *reinterpret_cast<const uint4*>(p + 64 * t);
+      for (int t = 0; t < KS; ++t) kr[u][t] = *reinterpret_cast<const u32x4*>(p + 64 * t);
     }
 #pragma unroll
     for (int i = 0; i < kVld; ++i) {
       const int s = __shfl(slot, i * kRpi + lane / kCpr, 64);
-      vr[i] = *reinterpret_cast<const uint4*>(vbase + max(s, 0) * pitch);
+      vr[i] = *reinterpret_cast<const u32x4*>(vbase + max(s, 0) * pitch);
     }
   };
 
-  f32x4 o[OT];
+  f32x4 o[RT][OT];
+  float m[RT], l[RT];  // m in log2 units; l: over this lane's keys
 #pragma unroll
-  for (int d = 0; d < OT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, l = 0.0f;  // m in log2 units; l: over this lane's keys
-  unsigned char* vb = buf[wave];
+  for (int x = 0; x < RT; ++x) {
+    m[x] = -INFINITY, l[x] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < OT; ++d) o[x][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
   const float neg1 = minus_one();
 
   constexpr int kStep = kWaves * kKeys;
-  int kb = k0 + wave * kKeys;
+  int kb = it.k0 + wave * kKeys;
   int slot = -1, entry = -1;
   if (kb < k1) {
     slot = slot_of(page_entry(kb), kb);
@@ -264,26 +352,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
   }
   for (; kb < k1; kb += kStep) {
     // S^T: keys 16 u + 4 quad + i, row r16
-    f32x4 s[2];
+    f32x4 s[RT][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      f32x4 lo = s[u];
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        s[u] = mfma16(__builtin_bit_cast(C8, kr[u][t]), qv[t], s[u]);
-        if constexpr (kSplit) lo = mfma16(__builtin_bit_cast(C8, kr[u][t]), ql[t], lo);
+      for (int u = 0; u < 2; ++u) {
+        s[x][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 lo = s[x][u];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+          s[x][u] = mfma16(__builtin_bit_cast(C8, kr[u][t]), qv[x][t], s[x][u]);
+          if constexpr (kSplit) lo = mfma16(__builtin_bit_cast(C8, kr[u][t]), ql[x][t], lo);
+        }
+        if constexpr (kSplit)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[x][u][i] += lo[i];
       }
-      if constexpr (kSplit)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][i] += lo[i];
-    }
     const uint32_t held = static_cast<uint32_t>(__ballot(slot >= 0));
 #pragma unroll
     for (int i = 0; i < kVld; ++i) {
       const int r = i * kRpi + lane / kCpr, c = lane % kCpr;
-      if (held != 0xffffffffu && !((held >> r) & 1)) vr[i] = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4)) = vr[i];
+      if (held != 0xffffffffu) vr[i] &= (held >> r) & 1 ? 0xffffffffu : 0u;
+      *reinterpret_cast<u32x4*>(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4)) = vr[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (kb + kStep < k1) {
@@ -291,49 +381,37 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
       load(slot);
       entry = page_entry(kb + 2 * kStep);
     }
-    if (held != 0xffffffffu || kb + kKeys > least) {
+    C8 ph[RT], pl[RT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int x = 0; x < RT; ++x) {
+      if (held != 0xffffffffu || kb + kKeys > least) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = 16 * u + 4 * quad + i;
-          if (kb + k >= lim || !((held >> k) & 1)) s[u][i] = -INFINITY;
-        }
-    }
-    float mb = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mb = swap_combine32<true>(swap_combine16<true>(mb)) * a.cs;
-    // the sums are rescaled only where a maximum has grown by more than 2^8: weights stay below that
-    if (__any(mb > m + 8.0f)) {
-      const float m_new = fmaxf(m, mb);
-      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      l *= alpha;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int d = 0; d < OT; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
-    }
-    const float mu = m == -INFINITY ? 0.0f : m;
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], a.cs, -mu));
-    C8 ph, pl;
-    if constexpr (kSplit) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) split_f16_pair(p[2 * i], p[2 * i + 1], neg1, hi[i], lo[i]);
-      ph = __builtin_bit_cast(C8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      pl = __builtin_bit_cast(C8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l += p[i];
-    } else {
-      // weights rounded to the cache's type; the sum is that of the rounded ones, so that a row's weights add to 1
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ph[i] = static_cast<C>(p[i]);
-        l += static_cast<float>(ph[i]);
+          for (int i = 0; i < 4; ++i) {
+            const int k = 16 * u + 4 * quad + i;
+            if (kb + k >= w[x].lim || !((held >> k) & 1)) s[x][u][i] = -INFINITY;
+          }
       }
+      float mb = max3(max3(s[x][0][0], s[x][0][1], s[x][0][2]), max3(s[x][0][3], s[x][1][0], s[x][1][1]),
+                      max3(s[x][1][2], s[x][1][3], s[x][1][3]));
+      mb = swap_combine32<true>(swap_combine16<true>(mb)) * a.cs;
+      // the sums are rescaled only where a maximum has grown by more than 2^8: weights stay below that
+      if (__any(mb > m[x] + 8.0f)) {
+        const float m_new = fmaxf(m[x], mb);
+        const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - m_new);
+        m[x] = m_new;
+        l[x] *= alpha;
+#pragma unroll
+        for (int d = 0; d < OT; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[x][d][i] *= alpha;
+      }
+      const float mu = m[x] == -INFINITY ? 0.0f : m[x];
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[x][i >> 2][i & 3], a.cs, -mu));
+      weights8<QT, CT>(p, neg1, &ph[x], &pl[x], &l[x]);
     }
 #pragma unroll
     for (int d = 0; d < OT; ++d) {
@@ -344,64 +422,322 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
         v[u] = read_tr4(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4) + (r16 & 1) * 8);
       }
       const C8 va = __builtin_bit_cast(C8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-      o[d] = mfma16(va, ph, o[d]);
-      if constexpr (kSplit) o[d] = mfma16(va, pl, o[d]);
+#pragma unroll
+      for (int x = 0; x < RT; ++x) {
+        o[x][d] = mfma16(va, ph[x], o[x][d]);
+        if constexpr (kSplit) o[x][d] = mfma16(va, pl[x], o[x][d]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 
   // Join the four waves: (m, l) of each, then the weighted o.
-  l = swap_combine32<false>(swap_combine16<false>(l));
-  if (l != l && m == -INFINITY) m = 0.0f;  // every score was NaN: not a range without keys
-  if (quad == 0) wml[wave][r16] = make_float2(m, l);
-  __syncthreads();
-  float M = wml[0][r16].x;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wml[w][r16].x);
-  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-  float* jb = reinterpret_cast<float*>(buf[wave]);
-  if (row_ok) {
+  for (int x = 0; x < RT; ++x) {
+    l[x] = swap_combine32<false>(swap_combine16<false>(l[x]));
+    if (l[x] != l[x] && m[x] == -INFINITY) m[x] = 0.0f;  // every score was NaN: not a range without keys
+    if (quad == 0) wml[wave][16 * x + r16] = make_float2(m[x], l[x]);
+  }
+  __syncthreads();
+  float* jb = reinterpret_cast<float*>(vb);
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    float M = wml[0][16 * x + r16].x;
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) M = fmaxf(M, wml[v][16 * x + r16].x);
+    const float f = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
+    if (w[x].ok) {
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+        *reinterpret_cast<f32x4*>(jb + (16 * x + r16) * kPitch + 16 * d + 4 * quad) =
+            f32x4{f * o[x][d][0], f * o[x][d][1], f * o[x][d][2], f * o[x][d][3]};
+    }
+  }
+  __syncthreads();
+  // thread: row r, dims 4 c ..; a row's place is that of lane r % 16 (all lanes take part in the shuffles: kC4 is 16 or 32)
+  constexpr int kC4 = HD / 4;
+#pragma unroll
+  for (int x = 0; x < RT; ++x)
+    for (int e = threadIdx.x; e < 16 * kC4; e += kThreads) {
+      const int r = e / kC4, c = e % kC4;
+      Row y;
+      y.token = __shfl(w[x].token, r, 64), y.head = __shfl(w[x].head, r, 64);
+      if (!__shfl(static_cast<int>(w[x].ok), r, 64)) continue;
+      float mm = wml[0][16 * x + r].x;
+#pragma unroll
+      for (int v = 1; v < kWaves; ++v) mm = fmaxf(mm, wml[v][16 * x + r].x);
+      float den = 0.0f;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float2 z = wml[i][16 * x + r];
+        den += z.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z.x - mm) * z.y;
+        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + i * kBuf) + (16 * x + r) * kPitch + 4 * c);
+      }
+      const float y4[4] = {v[0], v[1], v[2], v[3]};
+      store_o<QT, HD, 4>(a, y, it.part, 4 * c, y4, mm, den);
+    }
+}
+
+// Shared form: 32 RW rows of one KV head, 32 rows a wave; the waves share stages of 64 keys in LDS (two buffers, one
+// barrier a stage). With RW == 2 the two halves of the workgroup take the two 32-key blocks of a stage and join at the
+// end; with RW == 4 every wave takes both.
+//
+// Per block and wave: S^T = K Q^T by 32x32x16 MFMA (lane: one row, half of the keys), softmax as above, O^T += V^T P^T with
+// the accumulators of S^T as the operand: lane half h supplies keys 16 u + 8 (i / 4) + 4 h + i % 4, and the transposing
+// reads of V follow the same order. A stage goes from memory through registers (the loads of stage b + 1 are issued
+// before stage b is computed, and stored behind it), since rows come from any page and those without a key are
+// cleared on the way.
+template <int QT, int CT, int HD, int RW>
+__device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, unsigned char* lds, float2 (*wml)[64]) {
+  typedef vec8<CT> C8;
+  constexpr bool kSplit = QT == Q4_F32;
+  constexpr int KW = kWaves / RW;
+  constexpr int KS = HD / 16, OT = HD / 32;  // MFMA steps over the dims; 32-dim output tiles
+  constexpr int kRowB = HD * 2;
+  constexpr int kCpr = HD / 8;
+  constexpr int kHalf = kStage * kRowB;           // bytes of a stage's K (or V)
+  constexpr int kLd = kStage * kCpr / kThreads;   // K (and V) loads per thread
+  constexpr int kRpi = kThreads / kCpr;           // rows per load round
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, ql_ = lane & 31;
+  const int rw = wave % RW, kw = wave / RW;
+
+  const Row w = row_of(a, it, it.row0 + 32 * rw + ql_);
+  int most = w.lim, least = w.ok ? w.lim : INT32_MAX;
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) {
+    most = max(most, __shfl_xor(most, m, 64));
+    least = min(least, __shfl_xor(least, m, 64));
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+  C8 qv[KS], qlo[kSplit ? KS : 1];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w, 16 * t + 8 * half, &qv[t], &qlo[kSplit ? t : 0]);
+
+  // Stages: lane l of every wave looks up key kb + l; thread: rows i kRpi + tid / kCpr of the stage, chunk tid % kCpr.
+  const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
+  const int k1 = it.k1;
+  auto page_entry = [&](int kb) {
+    const int j = kb + lane;
+    return j < k1 ? pages[a.b.by_page.div(j)] : -1;
+  };
+  auto slot_of = [&](int entry, int kb) {
+    const int j = kb + lane;
+    return j < k1 ? a.b.slot(entry, j - a.b.by_page.div(j) * a.b.page_size) : -1;
+  };
+  const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
+  const int lr = threadIdx.x / kCpr, lc = threadIdx.x % kCpr;
+  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + 16 * lc;
+  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + 16 * lc;
+  u32x4 kr[kLd], vr[kLd];
+  auto load = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < kLd; ++i) {
+      const int64_t off = max(__shfl(slot, i * kRpi + lr, 64), 0) * pitch;
+      kr[i] = *reinterpret_cast<const u32x4*>(kbase + off);
+      vr[i] = *reinterpret_cast<const u32x4*>(vbase + off);
+    }
+  };
+  auto store = [&](int buf, uint64_t held) {
+    unsigned char* kd = lds + buf * 2 * kHalf;
+#pragma unroll
+    for (int i = 0; i < kLd; ++i) {
+      const int r = i * kRpi + lr;
+      if (held != ~uint64_t{0}) vr[i] &= (held >> r) & 1 ? 0xffffffffu : 0u;
+      *reinterpret_cast<u32x4*>(kd + r * kRowB + ((lc ^ kswz<HD>(r)) << 4)) = kr[i];
+      *reinterpret_cast<u32x4*>(kd + kHalf + r * kRowB + ((lc ^ vswz<HD>(r)) << 4)) = vr[i];
+    }
+  };
+
+  f32x16 o[OT];
+#pragma unroll
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  const float neg1 = minus_one();
+  const int kr4 = (lane & 15) >> 2;
+  const int vrow = (4 * half + kr4) * kRowB + (lane & 1) * 8;
+  int vcol[OT];
+#pragma unroll
+  for (int d = 0; d < OT; ++d) vcol[d] = vrow + (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz<HD>(kr4)) << 4);
+
+  auto compute = [&](const unsigned char* Ks, const unsigned char* Vs, int kb, uint32_t held) {
+    if (kb >= most) return;
+    f32x16 s = {}, s_lo = {};
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      const C8 ka = *reinterpret_cast<const C8*>(Ks + ql_ * kRowB + (((2 * t + half) ^ kswz<HD>(ql_)) << 4));
+      s = mfma32(ka, qv[t], s);
+      if constexpr (kSplit) s_lo = mfma32(ka, qlo[t], s_lo);
+    }
+    if constexpr (kSplit)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] += s_lo[e];
+    if (held != 0xffffffffu || kb + 32 > least) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = 8 * (e >> 2) + 4 * half + (e & 3);
+        if (kb + k >= w.lim || !((held >> k) & 1)) s[e] = -INFINITY;
+      }
+    }
+    float mb = max3(max3(max3(s[0], s[1], s[2]), s[3], s[4]), max3(max3(s[5], s[6], s[7]), s[8], s[9]),
+                    max3(max3(s[10], s[11], s[12]), max3(s[13], s[14], s[15]), s[15]));
+    mb = swap_combine32<true>(mb) * a.cs;
+    if (__any(mb > m + 8.0f)) {
+      const float m_new = fmaxf(m, mb);
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], a.cs, -mu));
+      C8 ph, pl;
+      weights8<QT, CT>(p, neg1, &ph, &pl, &l);
+      C8 va[OT];
+#pragma unroll
+      for (int d = 0; d < OT; ++d) {
+        const short4v v0 = read_tr4(Vs + vcol[d] + (16 * u) * kRowB);
+        const short4v v1 = read_tr4(Vs + vcol[d] + (16 * u + 8) * kRowB);
+        va[d] = __builtin_bit_cast(C8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+#pragma unroll
+      for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], ph, o[d]);
+      if constexpr (kSplit)
+#pragma unroll
+        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], pl, o[d]);
+    }
+  };
+
+  if (it.k0 < k1) {
+    int slot = slot_of(page_entry(it.k0), it.k0);
+    load(slot);
+    uint64_t held = __ballot(slot >= 0);
+    int entry = page_entry(it.k0 + kStage);
+    store(0, held);
+    __syncthreads();
+    int buf = 0;
+    for (int kb = it.k0; kb < k1; kb += kStage) {
+      const bool more = kb + kStage < k1;
+      if (more) {
+        slot = slot_of(entry, kb + kStage);
+        load(slot);
+        entry = page_entry(kb + 2 * kStage);
+      }
+      const unsigned char* Ks = lds + buf * 2 * kHalf;
+      if constexpr (KW == 2) {
+        compute(Ks + 32 * kw * kRowB, Ks + kHalf + 32 * kw * kRowB, kb + 32 * kw, static_cast<uint32_t>(held >> (32 * kw)));
+      } else {
+        compute(Ks, Ks + kHalf, kb, static_cast<uint32_t>(held));
+        compute(Ks + 32 * kRowB, Ks + kHalf + 32 * kRowB, kb + 32, static_cast<uint32_t>(held >> 32));
+      }
+      if (more) {
+        held = __ballot(slot >= 0);
+        store(buf ^ 1, held);
+      }
+      __syncthreads();  // stage b + 1 is written, and the buffer of stage b free
+      buf ^= 1;
+    }
+  }
+
+  l = swap_combine32<false>(l);
+  if (l != l && m == -INFINITY) m = 0.0f;
+  if constexpr (KW == 2) {
+    // the second half of the workgroup hands its rows over, register by register (the lanes hold the same places)
+    float* jb = reinterpret_cast<float*>(lds) + rw * OT * 16 * 64 + lane;
+    if (kw == 1) {
+      wml[rw][lane] = make_float2(m, l);
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) jb[(d * 16 + e) * 64] = o[d][e];
+    }
+    __syncthreads();
+    if (kw == 1) return;
+    const float2 x = wml[rw][lane];
+    const float M = fmaxf(m, x.x);
+    const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    const float f1 = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - M);
+    m = M;
+    l = f0 * l + f1 * x.y;
 #pragma unroll
     for (int d = 0; d < OT; ++d)
-      *reinterpret_cast<f32x4*>(jb + r16 * kPitch + 16 * d + 4 * quad) =
-          f32x4{f * o[d][0], f * o[d][1], f * o[d][2], f * o[d][3]};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = f0 * o[d][e] + f1 * jb[(d * 16 + e) * 64];
   }
-  __syncthreads();
-  // thread: row r, dims 4 c ..; a row's token and head are those of lane r
-  constexpr int kC4 = HD / 4;
-  const int part = shared ? split : a.shared_splits + split;
-  for (int e = threadIdx.x; e < kRows * kC4; e += kThreads) {
-    const int r = e / kC4, c = e % kC4;
-    // (kC4 is 16 or 32: every wave's lanes hold 4 or 2 rows, and all lanes take part in the shuffles)
-    const int rt = __shfl(token, r, 64), rh = __shfl(head, r, 64);
-    if (!__shfl(static_cast<int>(row_ok), r, 64)) continue;
-    float mm = wml[0][r].x;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, wml[w][r].x);
-    float den = 0.0f;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int d = 0; d < OT; ++d)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float2 x = wml[w][r];
-      den += x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - mm) * x.y;
-      v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf[w]) + r * kPitch + 4 * c);
+    for (int b = 0; b < 4; b += 2) {
+      // dims 8 b + 4 half + i and 8 (b + 1) + 4 half + i of the tile -> lane half h gets all of 8 (b + h) ..
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = o[d][4 * b + i], y = o[d][4 * b + 4 + i];
+        const auto t = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y),
+                                                        false, false);
+        const unsigned lo = t[0], hi = t[1];  // (a bit cast of a vector element reads element 0 with this compiler)
+        v[i] = __builtin_bit_cast(float, lo);
+        v[4 + i] = __builtin_bit_cast(float, hi);
+      }
+      if (w.ok) store_o<QT, HD, 8>(a, w, it.part, 32 * d + 8 * (b + half), v, m, l);
     }
-    const int64_t row = static_cast<int64_t>(rt) * a.n_q + rh;
-    if (a.parts == 1) {
-      const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-      Q y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = static_cast<Q>(v[i] * inv);
-      struct alignas(4 * sizeof(Q)) Q4v {
-        Q v[4];
-      };
-      *reinterpret_cast<Q4v*>(static_cast<Q*>(a.out) + row * HD + 4 * c) = Q4v{{y[0], y[1], y[2], y[3]}};
-    } else {
-      const int64_t i = row * a.parts + part;
-      *reinterpret_cast<f32x4*>(a.o + i * HD + 4 * c) = v;
-      if (c == 0) *reinterpret_cast<float2*>(a.ml + 2 * i) = make_float2(mm, den);
-    }
+}
+
+template <int QT, int CT, int HD>
+__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[lds_bytes(HD)];
+  __shared__ float2 wml[kWaves][64];
+  int idx = blockIdx.x;
+  Item it;
+  it.shared = idx < a.shared_blocks;
+  if (!it.shared) idx -= a.shared_blocks;
+  const int hs = a.by_kv.div(idx);
+  it.h = idx - hs * a.n_kv;
+  int tile = it.shared ? a.by_shared.div(hs) : a.by_own.div(hs), height;
+  const int split = hs - tile * (it.shared ? a.shared_splits : a.own_splits);
+  it.seq = 0, it.tok0 = 0, it.own_end = 0, it.behind = 0;
+  if (it.shared) {
+    height = a.shared_tile;
+    it.row0 = tile * height;
+    it.n_rows = a.T * a.g;
+    it.k0 = split * a.shared_keys;
+    it.k1 = min(it.k0 + a.shared_keys, a.shared_len);
+    it.part = split;
+  } else {
+    if (!own_tile(a, tile, QT == Q4_F32, &it.seq, &tile)) return;
+    it.seq = __builtin_amdgcn_readfirstlane(it.seq);
+    const int2 tk = tokens_of(a.b, it.seq, a.T);
+    it.tok0 = tk.x;
+    it.n_rows = tk.y * a.g;
+    height = tile_rows(it.n_rows, QT == Q4_F32);
+    it.row0 = tile * height;
+    it.own_end = min(a.b.keys(it.seq), a.L);
+    it.behind = a.b.lens[it.seq] - tk.y;
+    const int n = max(it.own_end - a.shared_len, 0);
+    const int per = ((n + a.own_splits - 1) / a.own_splits + kStage - 1) / kStage * kStage;
+    it.k0 = a.shared_len + min(split * per, n);
+    // no row of the tile sees more than its last
+    const int last = a.by_g.div(min(it.row0 + height, it.n_rows) - 1);
+    it.k1 = min(min(it.k0 + per, it.own_end), it.behind + last + 1);
+    it.part = a.shared_splits + split;
   }
+  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, lds, wml);
+  if constexpr (QT != Q4_F32)
+    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, lds, wml);
+  if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, lds, wml);
+  else paged_shared<QT, CT, HD, 4>(a, it, lds, wml);
 }
 
 // Joins the ranges of each row, a thread for 4 dims of a row; the first kB ranges are in flight at once.
@@ -448,7 +784,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
         for (int j = 0; j < 4; ++j) num[j] = fmaf(w, v[i][j], num[j]);
       }
   }
-  const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+  const float inv = den > 0.0f ? 1.0f / den : den;
   struct alignas(4 * sizeof(Q)) Q4v {
     Q v[4];
   };
@@ -460,25 +796,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
 
 struct Plan {
   int64_t shared_tiles, own_tiles;  // row tiles (own: an upper bound)
-  int shared_splits, shared_keys, own_splits, parts;
+  int shared_tile, shared_splits, shared_keys, own_splits, parts;
 };
 
-// Ranges: enough workgroups to give every compute unit two, and no range below 128 keys (a block for each wave).
+// Ranges: enough workgroups to give every compute unit two, and no range below 128 keys.
 int splits_for(int64_t items, int64_t keys) {
   const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(items, 1));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (keys + 127) / 128, 64})));
 }
 
-Plan plan_for(int64_t T, int g, int n_kv, int batch, bool ragged, int L, int shared_len) {
+Plan plan_for(int64_t T, int g, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
   Plan p{};
   const int64_t rows = T * g;
-  p.own_tiles = ragged ? (rows + static_cast<int64_t>(kRows - 1) * batch) / kRows
-                       : batch * ((rows / batch + kRows - 1) / kRows);
+  // of ragged rows: at most one tile that is not full a sequence, and a full one has 64 rows at least (of 129 .. 192 rows: three tiles)
+  p.own_tiles = ragged ? rows / 64 + batch : batch * static_cast<int64_t>(tiles_of(rows / batch, split));
   p.own_splits = L > shared_len ? splits_for(n_kv * p.own_tiles, L - shared_len) : 0;
   if (shared_len > 0) {
-    p.shared_tiles = (rows + kRows - 1) / kRows;
+    p.shared_tile = tile_rows(rows, split);
+    p.shared_tiles = tiles_of(rows, split);
     const int s = splits_for(n_kv * p.shared_tiles, shared_len);
-    p.shared_keys = ((shared_len + s - 1) / s + kKeys - 1) / kKeys * kKeys;
+    p.shared_keys = ((shared_len + s - 1) / s + kStage - 1) / kStage * kStage;
     p.shared_splits = (shared_len + p.shared_keys - 1) / p.shared_keys;
   }
   p.parts = p.shared_splits + p.own_splits;
@@ -516,9 +853,10 @@ extern "C" int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head
   if (!bytes) return Q4_ERR_NULL;
   if (int st = attn_args(T, n_q, n_kv, head_dim, batch, L, shared_len)) return st;
   size_t most = 0;
-  for (const bool ragged : {false, true}) {
+  for (const int form : {0, 1, 2, 3}) {  // cu_q or not, fp32 or not
+    const bool ragged = form & 1, split = form & 2;
     if (!ragged && T % batch) continue;
-    const Plan p = plan_for(T, n_q / n_kv, n_kv, batch, ragged, L, shared_len);
+    const Plan p = plan_for(T, n_q / n_kv, n_kv, batch, ragged, split, L, shared_len);
     const size_t n = static_cast<size_t>(T) * n_q * p.parts;
     if (p.parts > 1) most = std::max(most, (ml_floats(n) + n * head_dim) * sizeof(float));
   }
@@ -542,7 +880,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     return Q4_ERR_ALIGN;
   if (T == 0) return Q4_OK;
   const int g = n_q / kv->n_kv;
-  const Plan p = plan_for(T, g, kv->n_kv, kv->batch, kv->cu_q != nullptr, L, shared_len);
+  const Plan p = plan_for(T, g, kv->n_kv, kv->batch, kv->cu_q != nullptr, dtype == Q4_F32, L, shared_len);
   const size_t n = static_cast<size_t>(T) * n_q * p.parts;
   if (p.parts > 1) {
     if (!workspace || workspace_bytes < (ml_floats(n) + n * hd) * sizeof(float)) return Q4_ERR_WORKSPACE;
@@ -558,6 +896,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
   a.shared_pages = shared_pages;
   a.T = static_cast<int>(T), a.n_q = n_q, a.n_kv = kv->n_kv, a.g = g, a.L = L, a.shared_len = shared_len;
   a.shared_blocks = static_cast<int>(shared_blocks), a.shared_splits = p.shared_splits, a.shared_keys = p.shared_keys;
+  a.shared_tile = p.shared_tile;
   a.own_splits = p.own_splits, a.parts = p.parts;
   // a negative scale turns q around and a zero one clears it, so that the exponents' factor is positive
   a.sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
