@@ -22,7 +22,8 @@ def _left_to_python(*args):
 
 # The usual calls in native code: a call of q4_gemv 11.4 -> 5.0 us, of QLinear.forward at M = 1 16.8 -> 5.8.
 _NATIVE = native_calls()
-_gemv, linear_call, _attn, _gemm = (getattr(_NATIVE, n, _left_to_python) for n in ("gemv", "linear", "attn", "gemm"))
+_gemv, linear_call, _attn, _gemm, _rope, _append, _paged, _verify = (
+    getattr(_NATIVE, n, _left_to_python) for n in ("gemv", "linear", "attn", "gemm", "rope", "append", "paged", "verify"))
 
 
 def _dev(*ts):
@@ -434,6 +435,9 @@ _DT3 = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _CACHES = {torch.float32: torch.float16, torch.float16: torch.float16, torch.bfloat16: torch.bfloat16}
 
 
+_NO_ROPE = (None, False, 1.0)
+
+
 class _RopeC(C.Structure):
     """struct q4_rope of include/q4llm.h."""
     _fields_ = [("inv_freq", C.c_void_p), ("rot_dim", C.c_int), ("layout", C.c_int), ("mscale", C.c_float)]
@@ -501,6 +505,9 @@ def _paged_c(k_cache, v_cache, page_table, seq_lens, cu_q, dtype, tokens, n_kv=N
 def rope_rotate(x, positions, rope, inverse=False, out=None):
     """x [T, heads, hd] (fp32, fp16 or bf16, rows and heads may be strided) rotated at positions [T] (device int32) by
     `rope` (q4llm.rope.Rope); `inverse` rotates back (the gradient). `out` may be x."""
+    y = _rope(x, positions, *rope, inverse, out)
+    if y is not None:
+        return y
     if x.dim() != 3 or x.dtype not in _DT3:
         raise ValueError(f"x: expected [T, heads, hd] of float32, float16 or bfloat16, got {tuple(x.shape)} {x.dtype}")
     t, h, hd = x.shape
@@ -525,6 +532,9 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_q=None, rop
     seq_lens [batch] (this step's tokens included) and cu_q [batch + 1] (None: T / batch tokens each) are device int32.
     fp32 or fp16 with fp16 caches, bf16 with bf16 ones; operands may be strided (slices of a fused qkv row).
     Returns q_out (None without q)."""
+    y = _append(k, v, k_cache, v_cache, page_table, seq_lens, cu_q, *(_NO_ROPE if rope is None else rope), q, q_out)
+    if y is not None:
+        return None if y is True else y
     if k.dim() != 3:
         raise ValueError(f"k: expected [T, n_kv, hd], got {tuple(k.shape)}")
     t, n_kv, hd = k.shape
@@ -562,6 +572,9 @@ def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shar
     (device int32) for every sequence and are read once for the batch. L: no sequence has more keys (None: as
     many as a row of page_table holds; a lower bound gives shorter launches). The tokens past cu_q[-1] keep
     what `out` holds."""
+    y = _paged(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q, shared_pages, shared_len, L, workspace, out)
+    if y is not None:
+        return y
     if q.dim() != 3:
         raise ValueError(f"q: expected [T, n_q, hd], got {tuple(q.shape)}")
     t, n_q, hd = q.shape
@@ -604,6 +617,9 @@ def spec_verify(tokens, draft_probs, target_probs, uniforms, n_draft=None, works
     against target_probs [B, K + 1, V], with uniforms [B, K + 1] in [0, 1) (fp32) for the K acceptances and the
     next token; n_draft [B] int32: how many each row drafted (None: K). Returns (tokens [B, K + 1] int32: the
     accepted ones, the next one, then -1; accepted [B] int32). include/q4llm.h has the rule."""
+    y = _verify(tokens, draft_probs, target_probs, uniforms, n_draft, workspace)
+    if y is not None:
+        return y
     if tokens.dim() != 2 or target_probs.dim() != 3:
         raise ValueError(f"tokens {tuple(tokens.shape)}, target_probs {tuple(target_probs.shape)}: expected [B, K], [B, K + 1, V]")
     b, k = tokens.shape
