@@ -143,6 +143,14 @@ __device__ __forceinline__ int kswz(int r) {
   return HD == 128 ? (r & 15) : ((r >> 1) & 7);
 }
 
+// Row of the cache of key j from its page-list entry, -1 for none (past the end, or no page of the pool). No branch: one that
+// skips the use of a loaded entry makes the compiler wait for every load in flight before the register is written again.
+__device__ __forceinline__ int slot_at(const PagedBatch& b, int entry, int j, int end) {
+  const int s = entry * b.page_size + (j - b.by_page.div(max(j, 0)) * b.page_size);
+  const int bad = (entry >> 31) | ((b.num_pages - 1 - entry) >> 31) | ((end - 1 - j) >> 31);
+  return s | bad;
+}
+
 // What a workgroup does: the tile of rows, the keys k0 .. k1 - 1 of its range, and where the range's result goes.
 struct Item {
   bool shared;
@@ -209,6 +217,16 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const Row& w, int d, v
   }
 }
 
+// s + a + b of the two 16-bit values of w, in fp32.
+template <int CT>
+__device__ __forceinline__ float add_pair(uint32_t w, float s) {
+  typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
+  if constexpr (CT == Q4_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(C2, w), __builtin_bit_cast(C2, 0x3c003c00u), s, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(C2, w), __builtin_bit_cast(C2, 0x3f803f80u), s, false);
+}
+
 // Eight softmax weights as the B operand of P V: two fp16 terms with fp32 activations, else rounded to the cache's type; the
 // sum is that of what is multiplied, so that a row's weights add to 1.
 template <int QT, int CT>
@@ -223,13 +241,16 @@ __device__ __forceinline__ void weights8(const float (&p)[8], float neg1, vec8<C
 #pragma unroll
     for (int i = 0; i < 8; ++i) *sum += p[i];
   } else {
-    C8 r;
+    typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      r[i] = static_cast<typename Num<CT>::type>(p[i]);
-      *sum += static_cast<float>(r[i]);
+    for (int i = 0; i < 4; ++i) {
+      const C2 r = __builtin_convertvector((f32x2{p[2 * i], p[2 * i + 1]}), C2);
+      w[i] = __builtin_bit_cast(uint32_t, r);
+      *sum = add_pair<CT>(w[i], *sum);
     }
-    *hi_out = r;
+    *hi_out = __builtin_bit_cast(C8, make_uint4(w[0], w[1], w[2], w[3]));
   }
 }
 
@@ -256,8 +277,6 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Row& w, int par
   }
 }
 
-constexpr int lds_bytes(int HD) { return std::max(4 * kStage * HD * 2, kWaves * 32 * (HD + 4) * 4); }
-
 // Streaming form: 16 RT rows of one KV head, 32-key blocks dealt to the four waves, which keep (m, l, o) of their own and
 // join them at the end. What bounds it is the latency and bandwidth of the key loads.
 //
@@ -267,7 +286,8 @@ constexpr int lds_bytes(int HD) { return std::max(4 * kStage * HD * 2, kWaves * 
 // 4 quad + j - 4, and V^T comes from a row-major copy of the block in LDS in the same order by transposing reads.
 // The loads of the next block are issued when this one's registers are free, and cross its softmax and PV.
 template <int QT, int CT, int HD, int RT>
-__device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, unsigned char* lds, float2 (*wml)[64]) {
+__device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, unsigned char* buf0, unsigned char* buf1,
+                                             float2 (*wml)[64]) {
   typedef vec8<CT> C8;
   constexpr bool kSplit = QT == Q4_F32;      // q and P as two fp16 terms
   constexpr int KS = HD / 32, OT = HD / 16;  // MFMA steps over the dims; 16-dim output tiles
@@ -275,13 +295,13 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   constexpr int kCpr = HD / 8;               // 16-byte chunks per row
   constexpr int kVld = kKeys * kCpr / 64;    // V loads per lane
   constexpr int kRpi = 64 / kCpr;            // rows per load instruction
-  constexpr int kPitch = HD + 4;             // floats per row of the join buffer
-  constexpr int kBuf = 16 * RT * kPitch * 4; // of a wave: a V block, then its rows of o
-  static_assert(kBuf >= kKeys * kRowB && kWaves * kBuf <= lds_bytes(HD), "LDS of a wave");
+  constexpr int kBuf = 16 * RT * HD * 4;     // LDS of a wave (two waves a buffer): a V block, then its rows of o
+  static_assert(kBuf >= kKeys * kRowB && 2 * kBuf <= 2 * kStage * kRowB, "LDS of a wave");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, quad = lane >> 4;
-  unsigned char* vb = lds + wave * kBuf;
+  auto buf_of = [&](int wv) { return (wv < 2 ? buf0 : buf1) + (wv & 1) * kBuf; };
+  unsigned char* vb = buf_of(wave);
 
   Row w[RT];
   C8 qv[RT][KS], ql[RT][kSplit ? KS : 1];
@@ -302,17 +322,12 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   const int k1 = __builtin_amdgcn_readfirstlane(min(it.k1, most));
   least = __builtin_amdgcn_readfirstlane(least);
 
-  // Keys of a block: lane l (and l + 32) looks up key kb + l.
+  // Keys of a block: lane l (and l + 32) looks up key kb + l. The entry is loaded unconditionally, at the last key past the
+  // end: chosen or copied behind the key loads, it would wait for them all.
   const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
   const int kl = lane & 31;
-  auto page_entry = [&](int kb) {
-    const int j = kb + kl;
-    return j < k1 ? pages[a.b.by_page.div(j)] : -1;
-  };
-  auto slot_of = [&](int entry, int kb) {
-    const int j = kb + kl;
-    return j < k1 ? a.b.slot(entry, j - a.b.by_page.div(j) * a.b.page_size) : -1;
-  };
+  auto page_entry = [&](int kb) { return pages[a.b.by_page.div(min(kb + kl, k1 - 1))]; };
+  auto slot_of = [&](int entry, int kb) { return slot_at(a.b, entry, kb + kl, k1); };
   const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
   const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + 16 * quad;
   const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + 16 * (lane % kCpr);
@@ -376,11 +391,9 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
       *reinterpret_cast<u32x4*>(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4)) = vr[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (kb + kStep < k1) {
-      slot = slot_of(entry, kb + kStep);
-      load(slot);
-      entry = page_entry(kb + 2 * kStep);
-    }
+    slot = slot_of(entry, kb + kStep);
+    if (kb + kStep < k1) load(slot);
+    entry = page_entry(kb + 2 * kStep);
     C8 ph[RT], pl[RT];
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
@@ -439,7 +452,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     if (quad == 0) wml[wave][16 * x + r16] = make_float2(m[x], l[x]);
   }
   __syncthreads();
-  float* jb = reinterpret_cast<float*>(vb);
+  float* jb = reinterpret_cast<float*>(vb);  // rows of HD floats, their 16-byte chunks swizzled by the row
 #pragma unroll
   for (int x = 0; x < RT; ++x) {
     float M = wml[0][16 * x + r16].x;
@@ -449,7 +462,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     if (w[x].ok) {
 #pragma unroll
       for (int d = 0; d < OT; ++d)
-        *reinterpret_cast<f32x4*>(jb + (16 * x + r16) * kPitch + 16 * d + 4 * quad) =
+        *reinterpret_cast<f32x4*>(jb + (16 * x + r16) * HD + 4 * ((4 * d + quad) ^ r16)) =
             f32x4{f * o[x][d][0], f * o[x][d][1], f * o[x][d][2], f * o[x][d][3]};
     }
   }
@@ -472,12 +485,19 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
       for (int i = 0; i < kWaves; ++i) {
         const float2 z = wml[i][16 * x + r];
         den += z.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z.x - mm) * z.y;
-        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + i * kBuf) + (16 * x + r) * kPitch + 4 * c);
+        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf_of(i)) + (16 * x + r) * HD + 4 * (c ^ r));
       }
       const float y4[4] = {v[0], v[1], v[2], v[3]};
       store_o<QT, HD, 4>(a, y, it.part, 4 * c, y4, mm, den);
     }
 }
+
+// 16 bytes per lane from memory straight into LDS (lane i's at dst + 16 i).
+__device__ __forceinline__ void load_lds16(const unsigned char* src, unsigned char* dst) {
+  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(src),
+                                   (__attribute__((address_space(3))) void*)(dst), 16, 0, 0);
+}
+__device__ const uint4 kNoKey = {0, 0, 0, 0};  // what rows without a key read
 
 // Shared form: 32 RW rows of one KV head, 32 rows a wave; the waves share stages of 64 keys in LDS (two buffers, one
 // barrier a stage). With RW == 2 the two halves of the workgroup take the two 32-key blocks of a stage and join at the
@@ -485,20 +505,22 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
 //
 // Per block and wave: S^T = K Q^T by 32x32x16 MFMA (lane: one row, half of the keys), softmax as above, O^T += V^T P^T with
 // the accumulators of S^T as the operand: lane half h supplies keys 16 u + 8 (i / 4) + 4 h + i % 4, and the transposing
-// reads of V follow the same order. A stage goes from memory through registers (the loads of stage b + 1 are issued
-// before stage b is computed, and stored behind it), since rows come from any page and those without a key are
-// cleared on the way.
+// reads of V follow the same order. Stage b + 1 goes straight to LDS while stage b is computed: a row may come from any
+// page, one without a key from a row of zeros. The buffers are two LDS objects and the loop names them in turn, so
+// that the compiler sees that reads of one do not touch the loads into the other and does not wait for them.
 template <int QT, int CT, int HD, int RW>
-__device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, unsigned char* lds, float2 (*wml)[64]) {
+__device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, unsigned char* buf0, unsigned char* buf1,
+                                             float2 (*wml)[64]) {
   typedef vec8<CT> C8;
   constexpr bool kSplit = QT == Q4_F32;
   constexpr int KW = kWaves / RW;
-  constexpr int KS = HD / 16, OT = HD / 32;  // MFMA steps over the dims; 32-dim output tiles
+  constexpr int NB = KW == 1 && !kSplit ? 2 : 1;  // 32-key blocks of a wave at once (two terms: registers for one)
+  constexpr int KS = HD / 16, OT = HD / 32;       // MFMA steps over the dims; 32-dim output tiles
   constexpr int kRowB = HD * 2;
   constexpr int kCpr = HD / 8;
   constexpr int kHalf = kStage * kRowB;           // bytes of a stage's K (or V)
-  constexpr int kLd = kStage * kCpr / kThreads;   // K (and V) loads per thread
-  constexpr int kRpi = kThreads / kCpr;           // rows per load round
+  constexpr int kRpi = 64 / kCpr;                 // rows per load instruction of a wave
+  constexpr int kLd = kHalf / 1024 / kWaves;      // K (and V) load instructions per wave
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, ql_ = lane & 31;
@@ -517,38 +539,26 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
 #pragma unroll
   for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w, 16 * t + 8 * half, &qv[t], &qlo[kSplit ? t : 0]);
 
-  // Stages: lane l of every wave looks up key kb + l; thread: rows i kRpi + tid / kCpr of the stage, chunk tid % kCpr.
+  // Stages: lane l of every wave looks up key kb + l. Load instruction wave + 4 j fills rows (wave + 4 j) kRpi ..; the lane for
+  // chunk s of row r fetches chunk s ^ swz(r), the same for every j.
   const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
   const int k1 = it.k1;
-  auto page_entry = [&](int kb) {
-    const int j = kb + lane;
-    return j < k1 ? pages[a.b.by_page.div(j)] : -1;
-  };
-  auto slot_of = [&](int entry, int kb) {
-    const int j = kb + lane;
-    return j < k1 ? a.b.slot(entry, j - a.b.by_page.div(j) * a.b.page_size) : -1;
-  };
+  auto page_entry = [&](int kb) { return pages[a.b.by_page.div(min(kb + lane, k1 - 1))]; };
+  auto slot_of = [&](int entry, int kb) { return slot_at(a.b, entry, kb + lane, k1); };
   const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
-  const int lr = threadIdx.x / kCpr, lc = threadIdx.x % kCpr;
-  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + 16 * lc;
-  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + 16 * lc;
-  u32x4 kr[kLd], vr[kLd];
-  auto load = [&](int slot) {
+  const int lr = wave * kRpi + lane / kCpr, lc = lane % kCpr;
+  static_assert(kWaves * kRpi % 16 == 0, "one swizzle for all loads of a lane");
+  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + ((lc ^ kswz<HD>(lr)) << 4);
+  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + ((lc ^ vswz<HD>(lr)) << 4);
+  const unsigned char* none = reinterpret_cast<const unsigned char*>(&kNoKey);
+  auto issue = [&](unsigned char* buf, int slot) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kLd; ++i) {
-      const int64_t off = max(__shfl(slot, i * kRpi + lr, 64), 0) * pitch;
-      kr[i] = *reinterpret_cast<const u32x4*>(kbase + off);
-      vr[i] = *reinterpret_cast<const u32x4*>(vbase + off);
-    }
-  };
-  auto store = [&](int buf, uint64_t held) {
-    unsigned char* kd = lds + buf * 2 * kHalf;
-#pragma unroll
-    for (int i = 0; i < kLd; ++i) {
-      const int r = i * kRpi + lr;
-      if (held != ~uint64_t{0}) vr[i] &= (held >> r) & 1 ? 0xffffffffu : 0u;
-      *reinterpret_cast<u32x4*>(kd + r * kRowB + ((lc ^ kswz<HD>(r)) << 4)) = kr[i];
-      *reinterpret_cast<u32x4*>(kd + kHalf + r * kRowB + ((lc ^ vswz<HD>(r)) << 4)) = vr[i];
+    for (int j = 0; j < kLd; ++j) {
+      const int s = __shfl(slot, j * kWaves * kRpi + lr, 64);
+      const int64_t off = s * pitch;
+      unsigned char* dst = buf + (wave + j * kWaves) * 1024;
+      load_lds16(s < 0 ? none : kbase + off, dst);
+      load_lds16(s < 0 ? none : vbase + off, dst + kHalf);
     }
   };
 
@@ -565,27 +575,44 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
 #pragma unroll
   for (int d = 0; d < OT; ++d) vcol[d] = vrow + (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz<HD>(kr4)) << 4);
 
-  auto compute = [&](const unsigned char* Ks, const unsigned char* Vs, int kb, uint32_t held) {
+  // NB blocks from key row r0 of a stage on; kb: the first one's first key.
+  auto compute = [&](const unsigned char* buf, int r0, int kb, uint64_t held) __attribute__((always_inline)) {
     if (kb >= most) return;
-    f32x16 s = {}, s_lo = {};
+    const unsigned char* Ks = buf + r0 * kRowB;
+    const unsigned char* Vs = Ks + kHalf;
+    f32x16 s[NB];
+    C8 ka[NB][KS];
 #pragma unroll
-    for (int t = 0; t < KS; ++t) {
-      const C8 ka = *reinterpret_cast<const C8*>(Ks + ql_ * kRowB + (((2 * t + half) ^ kswz<HD>(ql_)) << 4));
-      s = mfma32(ka, qv[t], s);
-      if constexpr (kSplit) s_lo = mfma32(ka, qlo[t], s_lo);
-    }
-    if constexpr (kSplit)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] += s_lo[e];
-    if (held != 0xffffffffu || kb + 32 > least) {
+      for (int t = 0; t < KS; ++t)
+        ka[n][t] = *reinterpret_cast<const C8*>(Ks + (32 * n + ql_) * kRowB + (((2 * t + half) ^ kswz<HD>(ql_)) << 4));
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int k = 8 * (e >> 2) + 4 * half + (e & 3);
-        if (kb + k >= w.lim || !((held >> k) & 1)) s[e] = -INFINITY;
+    for (int n = 0; n < NB; ++n) {
+      s[n] = f32x16{};
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        if constexpr (kSplit) s[n] = mfma32(ka[n][t], qlo[t], s[n]);
+        s[n] = mfma32(ka[n][t], qv[t], s[n]);
       }
     }
-    float mb = max3(max3(max3(s[0], s[1], s[2]), s[3], s[4]), max3(max3(s[5], s[6], s[7]), s[8], s[9]),
-                    max3(max3(s[10], s[11], s[12]), max3(s[13], s[14], s[15]), s[15]));
+    if ((NB == 2 ? held != ~uint64_t{0} : static_cast<uint32_t>(held) != 0xffffffffu) || kb + 32 * NB > least) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int k = 32 * n + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (kb + k >= w.lim || !((held >> k) & 1)) s[n][e] = -INFINITY;
+        }
+    }
+    float mb = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float x = max3(max3(s[n][0], s[n][1], s[n][2]), s[n][3], s[n][4]);
+      const float y = max3(max3(s[n][5], s[n][6], s[n][7]), s[n][8], s[n][9]);
+      const float z = max3(max3(s[n][10], s[n][11], s[n][12]), max3(s[n][13], s[n][14], s[n][15]), mb);
+      mb = max3(x, y, z);
+    }
     mb = swap_combine32<true>(mb) * a.cs;
     if (__any(mb > m + 8.0f)) {
       const float m_new = fmaxf(m, mb);
@@ -599,55 +626,64 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
     }
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float p[8];
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], a.cs, -mu));
-      C8 ph, pl;
-      weights8<QT, CT>(p, neg1, &ph, &pl, &l);
-      C8 va[OT];
+      for (int u = 0; u < 2; ++u) {
+        float p[8];
 #pragma unroll
-      for (int d = 0; d < OT; ++d) {
-        const short4v v0 = read_tr4(Vs + vcol[d] + (16 * u) * kRowB);
-        const short4v v1 = read_tr4(Vs + vcol[d] + (16 * u + 8) * kRowB);
-        va[d] = __builtin_bit_cast(C8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[n][8 * u + i], a.cs, -mu));
+        C8 ph, pl;
+        weights8<QT, CT>(p, neg1, &ph, &pl, &l);
+        C8 va[OT];
+#pragma unroll
+        for (int d = 0; d < OT; ++d) {
+          const short4v v0 = read_tr4(Vs + vcol[d] + (32 * n + 16 * u) * kRowB);
+          const short4v v1 = read_tr4(Vs + vcol[d] + (32 * n + 16 * u + 8) * kRowB);
+          va[d] = __builtin_bit_cast(C8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], ph, o[d]);
+        if constexpr (kSplit)
+#pragma unroll
+          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], pl, o[d]);
       }
-#pragma unroll
-      for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], ph, o[d]);
-      if constexpr (kSplit)
-#pragma unroll
-        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], pl, o[d]);
-    }
   };
 
+  // All loads of this wave have landed and its reads are done; then all waves'.
+  auto turn = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(7 << 4);  // vmcnt(0), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
   if (it.k0 < k1) {
     int slot = slot_of(page_entry(it.k0), it.k0);
-    load(slot);
-    uint64_t held = __ballot(slot >= 0);
+    issue(buf0, slot);
     int entry = page_entry(it.k0 + kStage);
-    store(0, held);
-    __syncthreads();
-    int buf = 0;
-    for (int kb = it.k0; kb < k1; kb += kStage) {
+    int kb = it.k0;
+    uint64_t held = __ballot(slot >= 0);
+    // one stage from `cur` while the next one goes to `nxt`; false: it was the last
+    auto stage = [&](unsigned char* cur, unsigned char* nxt) __attribute__((always_inline)) {
+      const uint64_t now = held;
       const bool more = kb + kStage < k1;
-      if (more) {
-        slot = slot_of(entry, kb + kStage);
-        load(slot);
-        entry = page_entry(kb + 2 * kStage);
-      }
-      const unsigned char* Ks = lds + buf * 2 * kHalf;
+      slot = slot_of(entry, kb + kStage);
+      if (more) issue(nxt, slot);
+      entry = page_entry(kb + 2 * kStage);
+      held = __ballot(slot >= 0);
       if constexpr (KW == 2) {
-        compute(Ks + 32 * kw * kRowB, Ks + kHalf + 32 * kw * kRowB, kb + 32 * kw, static_cast<uint32_t>(held >> (32 * kw)));
+        compute(cur, 32 * kw, kb + 32 * kw, now >> (32 * kw));
+      } else if constexpr (NB == 2) {
+        compute(cur, 0, kb, now);
       } else {
-        compute(Ks, Ks + kHalf, kb, static_cast<uint32_t>(held));
-        compute(Ks + 32 * kRowB, Ks + kHalf + 32 * kRowB, kb + 32, static_cast<uint32_t>(held >> 32));
+        compute(cur, 0, kb, now);
+        compute(cur, 32, kb + 32, now >> 32);
       }
-      if (more) {
-        held = __ballot(slot >= 0);
-        store(buf ^ 1, held);
-      }
-      __syncthreads();  // stage b + 1 is written, and the buffer of stage b free
-      buf ^= 1;
+      kb += kStage;
+      turn();
+      return more;
+    };
+    turn();
+    while (stage(buf0, buf1) && stage(buf1, buf0)) {
     }
   }
 
@@ -655,7 +691,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
   if (l != l && m == -INFINITY) m = 0.0f;
   if constexpr (KW == 2) {
     // the second half of the workgroup hands its rows over, register by register (the lanes hold the same places)
-    float* jb = reinterpret_cast<float*>(lds) + rw * OT * 16 * 64 + lane;
+    float* jb = reinterpret_cast<float*>(buf0) + rw * OT * 16 * 64 + lane;
     if (kw == 1) {
       wml[rw][lane] = make_float2(m, l);
 #pragma unroll
@@ -697,7 +733,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
 
 template <int QT, int CT, int HD>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[lds_bytes(HD)];
+  __shared__ __attribute__((aligned(16))) unsigned char buf0[2 * kStage * HD * 2], buf1[2 * kStage * HD * 2];
   __shared__ float2 wml[kWaves][64];
   int idx = blockIdx.x;
   Item it;
@@ -733,11 +769,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     it.k1 = min(min(it.k0 + per, it.own_end), it.behind + last + 1);
     it.part = a.shared_splits + split;
   }
-  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, lds, wml);
+  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, buf0, buf1, wml);
   if constexpr (QT != Q4_F32)
-    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, lds, wml);
-  if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, lds, wml);
-  else paged_shared<QT, CT, HD, 4>(a, it, lds, wml);
+    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, buf0, buf1, wml);
+  if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, buf0, buf1, wml);
+  else paged_shared<QT, CT, HD, 4>(a, it, buf0, buf1, wml);
 }
 
 // Joins the ranges of each row, a thread for 4 dims of a row; the first kB ranges are in flight at once.

@@ -436,6 +436,18 @@ def test_paged_attn_nan_stays_in_its_row(dev):
         b.check(q, 1.0)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 20, 40])
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_paged_attn_many_small_weights(dev, dt, rows):
+    """One key far above thousands of others: weights below fp16's normal range (2^-14) carry most of the sum."""
+    b = Batch(dev, dt, 64, 1, 16, [3000], [rows], 2000, seed=rows)
+    q = torch.ones(rows, 2, 64).to(dt).to(dev)
+    b.k.copy_(torch.where(b.k.isnan(), b.k, torch.full_like(b.k, 0.25)))
+    first = b.shared_pages[0]
+    b.k[first, 3] = 0.25 + 10.5 / 8  # scores 2 and 2 + 10.5
+    b.check(q, 0.125)
+
+
 def test_paged_attn_cache_past_32_bits(dev):
     """Rows at byte offsets past 2^32 (and past 2^31 elements)."""
     n_kv, hd, page = 8, 128, 16
