@@ -19,6 +19,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kKeys = 32;   // keys of a wave's block (streaming form)
 constexpr int kStage = 64;  // keys of a workgroup's stage (shared form)
+constexpr int kTurn = kWaves * kKeys;  // keys that the waves of the streaming form take side by side
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -60,9 +61,8 @@ struct AttnArgs {
   float *ml, *o;  // ranges' (m, l) and o of each row: [T * n_q][parts]
   const int32_t* shared_pages;
   int T, n_q, n_kv, g, L, shared_len;
-  int shared_blocks, shared_splits, shared_keys;  // workgroups of the shared ranges, ranges, keys of a range
-  int shared_tile;                                // rows of a shared workgroup
-  int own_splits, parts;
+  int shared_blocks, shared_splits, shared_tile;  // workgroups of the shared ranges, ranges, rows of a workgroup
+  int own_from, own_splits, parts;                // own ranges: their first key, how many at most
   float cs, sign;  // exponents are s * cs in log2 units; sign: that of the scale, taken into q
   FastDiv by_g, by_kv, by_shared, by_own;
 };
@@ -151,13 +151,28 @@ __device__ __forceinline__ int slot_at(const PagedBatch& b, int entry, int j, in
   return s | bad;
 }
 
-// What a workgroup does: the tile of rows, the keys k0 .. k1 - 1 of its range, and where the range's result goes.
+// Address of row s of the cache (row 0 where there is none): one multiplication of 32 by 32 bits into 64.
+__device__ __forceinline__ const unsigned char* row_at(const unsigned char* base, int s, uint32_t pitch) {
+  return base + static_cast<uint64_t>(static_cast<uint32_t>(max(s, 0))) * pitch;
+}
+
+// What a workgroup does: the tile of rows, the keys of its range, and where the range's result goes. Ranges are dealt, not cut:
+// range s of n has the blocks s, s + n, .. of the keys (of `turn` keys, as many as a workgroup takes at once), so that its first
+// keys, and their page entries, are known before the length of the sequence is.
 struct Item {
   bool shared;
   int h, seq, row0, n_rows, tok0, part;  // rows row0 .. of the n_rows that start at token tok0
-  int k0, k1, own_end;                   // own_end: the keys of the sequence (own ranges)
+  int k0, step, k1;                      // blocks at k0, k0 + step, .. below k1
+  int own_end;                           // the keys of the sequence (own ranges)
+  const int32_t* table;                  // its row of the page table
   int behind;                            // own ranges: position of a token = behind + its index in the sequence
 };
+
+// The page-list entry of key j: of the shared keys, or of the sequence's own (past its list: its last entry).
+__device__ __forceinline__ int page_at(const AttnArgs& a, const Item& it, int j) {
+  const int p = a.b.by_page.div(j);
+  return j < a.shared_len ? a.shared_pages[p] : it.table[min(p, a.b.max_pages - 1)];
+}
 
 // One row: its token and head, and how many keys of the range's kind it sees (0: none, or no row). Wave-uniform flow.
 struct Row {
@@ -176,7 +191,7 @@ __device__ __forceinline__ Row row_of(const AttnArgs& a, const Item& it, int r) 
     if (w.ok && s < a.b.batch) {
       const int2 tk = tokens_of(a.b, s, a.T);
       w.ok = w.token >= tk.x && w.token < tk.x + tk.y;
-      w.lim = min(min(a.b.lens[s] - tk.y + (w.token - tk.x) + 1, a.b.keys(s)), a.shared_len);
+      w.lim = min(min(a.b.lens[s] - tk.y + (w.token - tk.x) + 1, a.b.keys_of(a.b.lens[s])), a.shared_len);
     } else {
       w.ok = false;
     }
@@ -286,8 +301,8 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Row& w, int par
 // 4 quad + j - 4, and V^T comes from a row-major copy of the block in LDS in the same order by transposing reads.
 // The loads of the next block are issued when this one's registers are free, and cross its softmax and PV.
 template <int QT, int CT, int HD, int RT>
-__device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, unsigned char* buf0, unsigned char* buf1,
-                                             float2 (*wml)[64]) {
+__device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, int entry, unsigned char* buf0,
+                                             unsigned char* buf1, float2 (*wml)[64]) {
   typedef vec8<CT> C8;
   constexpr bool kSplit = QT == Q4_F32;      // q and P as two fp16 terms
   constexpr int KS = HD / 32, OT = HD / 16;  // MFMA steps over the dims; 16-dim output tiles
@@ -303,32 +318,14 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   auto buf_of = [&](int wv) { return (wv < 2 ? buf0 : buf1) + (wv & 1) * kBuf; };
   unsigned char* vb = buf_of(wave);
 
-  Row w[RT];
-  C8 qv[RT][KS], ql[RT][kSplit ? KS : 1];
-  int most = 0, least = INT32_MAX;  // the keys any row sees; those that every row sees
-#pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    w[x] = row_of(a, it, it.row0 + 16 * x + r16);
-    most = max(most, w[x].lim);
-    if (w[x].ok) least = min(least, w[x].lim);
-#pragma unroll
-    for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w[x], 32 * t + 8 * quad, &qv[x][t], &ql[x][kSplit ? t : 0]);
-  }
-#pragma unroll
-  for (int m = 8; m >= 1; m >>= 1) {
-    most = max(most, __shfl_xor(most, m, 64));
-    least = min(least, __shfl_xor(least, m, 64));
-  }
-  const int k1 = __builtin_amdgcn_readfirstlane(min(it.k1, most));
-  least = __builtin_amdgcn_readfirstlane(least);
+  const int k1 = it.k1;
 
   // Keys of a block: lane l (and l + 32) looks up key kb + l. The entry is loaded unconditionally, at the last key past the
   // end: chosen or copied behind the key loads, it would wait for them all.
-  const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
   const int kl = lane & 31;
-  auto page_entry = [&](int kb) { return pages[a.b.by_page.div(min(kb + kl, k1 - 1))]; };
+  auto page_entry = [&](int kb) { return page_at(a, it, min(kb + kl, k1 - 1)); };
   auto slot_of = [&](int entry, int kb) { return slot_at(a.b, entry, kb + kl, k1); };
-  const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
+  const uint32_t pitch = static_cast<uint32_t>(a.n_kv) * kRowB;
   const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + 16 * quad;
   const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + 16 * (lane % kCpr);
   u32x4 kr[2][KS], vr[kVld];
@@ -336,16 +333,38 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int s = __shfl(slot, 16 * u + r16, 64);
-      const unsigned char* p = kbase + max(s, 0) * pitch;
+      const unsigned char* p = row_at(kbase, s, pitch);
 #pragma unroll
       for (int t = 0; t < KS; ++t) kr[u][t] = *reinterpret_cast<const u32x4*>(p + 64 * t);
     }
 #pragma unroll
     for (int i = 0; i < kVld; ++i) {
       const int s = __shfl(slot, i * kRpi + lane / kCpr, 64);
-      vr[i] = *reinterpret_cast<const u32x4*>(vbase + max(s, 0) * pitch);
+      vr[i] = *reinterpret_cast<const u32x4*>(row_at(vbase, s, pitch));
     }
   };
+
+  int kb = it.k0 + wave * kKeys;
+  int slot = slot_of(entry, kb);
+  if (kb < k1) {
+    load(slot);
+    entry = page_entry(kb + it.step);
+  }
+
+  // The rows, while the first keys are on their way.
+  Row w[RT];
+  C8 qv[RT][KS], ql[RT][kSplit ? KS : 1];
+  int least = INT32_MAX;  // the keys that every row sees
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    w[x] = row_of(a, it, it.row0 + 16 * x + r16);
+    if (w[x].ok) least = min(least, w[x].lim);
+#pragma unroll
+    for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w[x], 32 * t + 8 * quad, &qv[x][t], &ql[x][kSplit ? t : 0]);
+  }
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) least = min(least, __shfl_xor(least, m, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
 
   f32x4 o[RT][OT];
   float m[RT], l[RT];  // m in log2 units; l: over this lane's keys
@@ -357,15 +376,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   }
   const float neg1 = minus_one();
 
-  constexpr int kStep = kWaves * kKeys;
-  int kb = it.k0 + wave * kKeys;
-  int slot = -1, entry = -1;
-  if (kb < k1) {
-    slot = slot_of(page_entry(kb), kb);
-    load(slot);
-    entry = page_entry(kb + kStep);
-  }
-  for (; kb < k1; kb += kStep) {
+  for (; kb < k1; kb += it.step) {
     // S^T: keys 16 u + 4 quad + i, row r16
     f32x4 s[RT][2];
 #pragma unroll
@@ -391,9 +402,9 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
       *reinterpret_cast<u32x4*>(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4)) = vr[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    slot = slot_of(entry, kb + kStep);
-    if (kb + kStep < k1) load(slot);
-    entry = page_entry(kb + 2 * kStep);
+    slot = slot_of(entry, kb + it.step);
+    if (kb + it.step < k1) load(slot);
+    entry = page_entry(kb + 2 * it.step);
     C8 ph[RT], pl[RT];
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
@@ -497,7 +508,6 @@ __device__ __forceinline__ void load_lds16(const unsigned char* src, unsigned ch
   __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(src),
                                    (__attribute__((address_space(3))) void*)(dst), 16, 0, 0);
 }
-__device__ const uint4 kNoKey = {0, 0, 0, 0};  // what rows without a key read
 
 // Shared form: 32 RW rows of one KV head, 32 rows a wave; the waves share stages of 64 keys in LDS (two buffers, one
 // barrier a stage). With RW == 2 the two halves of the workgroup take the two 32-key blocks of a stage and join at the
@@ -506,11 +516,12 @@ __device__ const uint4 kNoKey = {0, 0, 0, 0};  // what rows without a key read
 // Per block and wave: S^T = K Q^T by 32x32x16 MFMA (lane: one row, half of the keys), softmax as above, O^T += V^T P^T with
 // the accumulators of S^T as the operand: lane half h supplies keys 16 u + 8 (i / 4) + 4 h + i % 4, and the transposing
 // reads of V follow the same order. Stage b + 1 goes straight to LDS while stage b is computed: a row may come from any
-// page, one without a key from a row of zeros. The buffers are two LDS objects and the loop names them in turn, so
+// page; those without a key read row 0 and have their values cleared in LDS before the stage is used (what lies
+// there may be NaN, and a weight of zero does not undo that). The buffers are two LDS objects and the loop names them in turn, so
 // that the compiler sees that reads of one do not touch the loads into the other and does not wait for them.
 template <int QT, int CT, int HD, int RW>
-__device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, unsigned char* buf0, unsigned char* buf1,
-                                             float2 (*wml)[64]) {
+__device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, int entry, unsigned char* buf0,
+                                             unsigned char* buf1, float2 (*wml)[64]) {
   typedef vec8<CT> C8;
   constexpr bool kSplit = QT == Q4_F32;
   constexpr int KW = kWaves / RW;
@@ -526,6 +537,32 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
   const int half = lane >> 5, ql_ = lane & 31;
   const int rw = wave % RW, kw = wave / RW;
 
+  // Stages: lane l of every wave looks up key kb + l. Load instruction wave + 4 j fills rows (wave + 4 j) kRpi ..; the lane for
+  // chunk s of row r fetches chunk s ^ swz(r), the same for every j.
+  const int k1 = it.k1;
+  auto page_entry = [&](int kb) { return page_at(a, it, min(kb + lane, k1 - 1)); };
+  auto slot_of = [&](int entry, int kb) { return slot_at(a.b, entry, kb + lane, k1); };
+  const uint32_t pitch = static_cast<uint32_t>(a.n_kv) * kRowB;
+  const int lr = wave * kRpi + lane / kCpr, lc = lane % kCpr;
+  static_assert(kWaves * kRpi % 16 == 0, "one swizzle for all loads of a lane");
+  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + ((lc ^ kswz<HD>(lr)) << 4);
+  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + ((lc ^ vswz<HD>(lr)) << 4);
+  auto issue = [&](unsigned char* buf, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kLd; ++j) {
+      const int s = __shfl(slot, j * kWaves * kRpi + lr, 64);
+      unsigned char* dst = buf + (wave + j * kWaves) * 1024;
+      load_lds16(row_at(kbase, s, pitch), dst);
+      load_lds16(row_at(vbase, s, pitch), dst + kHalf);
+    }
+  };
+
+  int slot = slot_of(entry, it.k0);
+  if (it.k0 < k1) {
+    issue(buf0, slot);
+    entry = page_entry(it.k0 + it.step);
+  }
+  // The rows, while the first stage is on its way.
   const Row w = row_of(a, it, it.row0 + 32 * rw + ql_);
   int most = w.lim, least = w.ok ? w.lim : INT32_MAX;
 #pragma unroll
@@ -538,29 +575,6 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
   C8 qv[KS], qlo[kSplit ? KS : 1];
 #pragma unroll
   for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w, 16 * t + 8 * half, &qv[t], &qlo[kSplit ? t : 0]);
-
-  // Stages: lane l of every wave looks up key kb + l. Load instruction wave + 4 j fills rows (wave + 4 j) kRpi ..; the lane for
-  // chunk s of row r fetches chunk s ^ swz(r), the same for every j.
-  const int32_t* pages = it.shared ? a.shared_pages : a.b.table + it.seq * a.b.stride;
-  const int k1 = it.k1;
-  auto page_entry = [&](int kb) { return pages[a.b.by_page.div(min(kb + lane, k1 - 1))]; };
-  auto slot_of = [&](int entry, int kb) { return slot_at(a.b, entry, kb + lane, k1); };
-  const int64_t pitch = static_cast<int64_t>(a.n_kv) * kRowB;
-  const int lr = wave * kRpi + lane / kCpr, lc = lane % kCpr;
-  static_assert(kWaves * kRpi % 16 == 0, "one swizzle for all loads of a lane");
-  const unsigned char* kbase = static_cast<const unsigned char*>(a.kc) + it.h * kRowB + ((lc ^ kswz<HD>(lr)) << 4);
-  const unsigned char* vbase = static_cast<const unsigned char*>(a.vc) + it.h * kRowB + ((lc ^ vswz<HD>(lr)) << 4);
-  const unsigned char* none = reinterpret_cast<const unsigned char*>(&kNoKey);
-  auto issue = [&](unsigned char* buf, int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < kLd; ++j) {
-      const int s = __shfl(slot, j * kWaves * kRpi + lr, 64);
-      const int64_t off = s * pitch;
-      unsigned char* dst = buf + (wave + j * kWaves) * 1024;
-      load_lds16(s < 0 ? none : kbase + off, dst);
-      load_lds16(s < 0 ? none : vbase + off, dst + kHalf);
-    }
-  };
 
   f32x16 o[OT];
 #pragma unroll
@@ -657,18 +671,20 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
     asm volatile("" ::: "memory");
   };
   if (it.k0 < k1) {
-    int slot = slot_of(page_entry(it.k0), it.k0);
-    issue(buf0, slot);
-    int entry = page_entry(it.k0 + kStage);
     int kb = it.k0;
     uint64_t held = __ballot(slot >= 0);
     // one stage from `cur` while the next one goes to `nxt`; false: it was the last
     auto stage = [&](unsigned char* cur, unsigned char* nxt) __attribute__((always_inline)) {
       const uint64_t now = held;
-      const bool more = kb + kStage < k1;
-      slot = slot_of(entry, kb + kStage);
+      const bool more = kb + it.step < k1;
+      if (now != ~uint64_t{0}) {
+        for (int i = threadIdx.x; i < kStage * kCpr; i += kThreads)
+          if (!((now >> (i / kCpr)) & 1)) reinterpret_cast<u32x4*>(cur + kHalf)[i] = u32x4{0, 0, 0, 0};
+        turn();
+      }
+      slot = slot_of(entry, kb + it.step);
       if (more) issue(nxt, slot);
-      entry = page_entry(kb + 2 * kStage);
+      entry = page_entry(kb + 2 * it.step);
       held = __ballot(slot >= 0);
       if constexpr (KW == 2) {
         compute(cur, 32 * kw, kb + 32 * kw, now >> (32 * kw));
@@ -678,7 +694,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
         compute(cur, 0, kb, now);
         compute(cur, 32, kb + 32, now >> 32);
       }
-      kb += kStage;
+      kb += it.step;
       turn();
       return more;
     };
@@ -686,7 +702,6 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
     while (stage(buf0, buf1) && stage(buf1, buf0)) {
     }
   }
-
   l = swap_combine32<false>(l);
   if (l != l && m == -INFINITY) m = 0.0f;
   if constexpr (KW == 2) {
@@ -743,14 +758,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
   it.h = idx - hs * a.n_kv;
   int tile = it.shared ? a.by_shared.div(hs) : a.by_own.div(hs), height;
   const int split = hs - tile * (it.shared ? a.shared_splits : a.own_splits);
-  it.seq = 0, it.tok0 = 0, it.own_end = 0, it.behind = 0;
+  it.seq = 0, it.tok0 = 0, it.own_end = 0, it.behind = 0, it.table = a.b.table;
   if (it.shared) {
     height = a.shared_tile;
-    it.row0 = tile * height;
     it.n_rows = a.T * a.g;
-    it.k0 = split * a.shared_keys;
-    it.k1 = min(it.k0 + a.shared_keys, a.shared_len);
-    it.part = split;
   } else {
     if (!own_tile(a, tile, QT == Q4_F32, &it.seq, &tile)) return;
     it.seq = __builtin_amdgcn_readfirstlane(it.seq);
@@ -758,68 +769,107 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     it.tok0 = tk.x;
     it.n_rows = tk.y * a.g;
     height = tile_rows(it.n_rows, QT == Q4_F32);
-    it.row0 = tile * height;
-    it.own_end = min(a.b.keys(it.seq), a.L);
-    it.behind = a.b.lens[it.seq] - tk.y;
-    const int n = max(it.own_end - a.shared_len, 0);
-    const int per = ((n + a.own_splits - 1) / a.own_splits + kStage - 1) / kStage * kStage;
-    it.k0 = a.shared_len + min(split * per, n);
+    it.table += it.seq * a.b.stride;
+  }
+  const bool stream = height <= 32;
+  const int turn = stream ? kTurn : kStage;
+  it.row0 = tile * height;
+  it.k0 = (it.shared ? 0 : a.own_from) + split * turn;
+  const int first = it.k0 + (stream ? threadIdx.x >> 6 << 5 | (threadIdx.x & 31) : threadIdx.x & 63);
+  const int entry = page_at(a, it, it.shared ? min(first, a.shared_len - 1) : max(first, 0));
+  if (it.shared) {
+    it.step = a.shared_splits * turn;
+    it.k1 = a.shared_len;
+    it.part = split;
+  } else {
+    const int len = a.b.lens[it.seq], tokens = a.b.cu ? it.n_rows / a.g : a.b.rows;
+    it.own_end = min(a.b.keys_of(len), a.L);
+    it.behind = len - tokens;
     // no row of the tile sees more than its last
     const int last = a.by_g.div(min(it.row0 + height, it.n_rows) - 1);
-    it.k1 = min(min(it.k0 + per, it.own_end), it.behind + last + 1);
+    it.k1 = min(it.own_end, it.behind + last + 1);
+    const int n = it.own_end - a.own_from;
+    const int ranges = min(a.own_splits, max((n + kTurn - 1) / kTurn, 1));
+    it.step = ranges * turn;
+    if (split >= ranges) it.k1 = it.k0;
     it.part = a.shared_splits + split;
   }
-  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, buf0, buf1, wml);
+  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, entry, buf0, buf1, wml);
   if constexpr (QT != Q4_F32)
-    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, buf0, buf1, wml);
-  if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, buf0, buf1, wml);
-  else paged_shared<QT, CT, HD, 4>(a, it, buf0, buf1, wml);
+    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, entry, buf0, buf1, wml);
+  if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, entry, buf0, buf1, wml);
+  else paged_shared<QT, CT, HD, 4>(a, it, entry, buf0, buf1, wml);
 }
 
-// Joins the ranges of each row, a thread for 4 dims of a row; the first kB ranges are in flight at once.
-template <int QT, int HD>
+// Joins the ranges of each row: PG threads, each for every PG-th range, and those side by side for 4 dims of the row; the first
+// kB ranges of a thread are in flight at once.
+template <int QT, int HD, int PG>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
   typedef typename Num<QT>::type Q;
-  constexpr int kC4 = HD / 4, kB = 8;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t row = e / kC4;
-  const int c = static_cast<int>(e % kC4);
-  if (row >= static_cast<int64_t>(a.T) * a.n_q) return;
+  constexpr int kC4 = HD / 4, kB = 4, kRow = kC4 * PG, kRowsWg = 256 / kRow;
+  __shared__ float sm[kRowsWg][PG][kC4], sd[kRowsWg][PG][kC4];
+  __shared__ f32x4 so[kRowsWg][PG][kC4];
+  const int lr = threadIdx.x / kRow, pg = threadIdx.x % kRow / kC4, c = threadIdx.x % kC4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsWg + lr;
+  bool ok = row < static_cast<int64_t>(a.T) * a.n_q;
   if (a.b.cu) {
     const int64_t t = row / a.n_q;
-    if (t < a.b.cu[0] || t >= a.b.cu[a.b.batch]) return;  // of no sequence
+    ok = ok && t >= a.b.cu[0] && t < a.b.cu[a.b.batch];  // else of no sequence
   }
   const float2* ml = reinterpret_cast<const float2*>(a.ml) + row * a.parts;
   const float* o = a.o + row * a.parts * HD + 4 * c;
   float M = -INFINITY, den = 0.0f;
   f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p0 = 0; p0 < a.parts; p0 += kB) {
-    float2 x[kB];
-    f32x4 v[kB];
+  if (ok)
+    for (int p0 = pg; p0 < a.parts; p0 += kB * PG) {
+      float2 x[kB];
+      f32x4 v[kB];
 #pragma unroll
-    for (int i = 0; i < kB; ++i) {
-      x[i] = make_float2(-INFINITY, 0.0f);
-      if (p0 + i < a.parts) {
-        x[i] = ml[p0 + i];
-        v[i] = *reinterpret_cast<const f32x4*>(o + static_cast<int64_t>(p0 + i) * HD);
+      for (int i = 0; i < kB; ++i) {
+        x[i] = make_float2(-INFINITY, 0.0f);
+        if (p0 + i * PG < a.parts) {
+          x[i] = ml[p0 + i * PG];
+          v[i] = *reinterpret_cast<const f32x4*>(o + static_cast<int64_t>(p0 + i * PG) * HD);
+        }
       }
+      float mb = M;
+#pragma unroll
+      for (int i = 0; i < kB; ++i) mb = fmaxf(mb, x[i].x);
+      const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+      M = mb;
+      den *= alpha;
+      num *= alpha;
+#pragma unroll
+      for (int i = 0; i < kB; ++i)
+        if (x[i].x != -INFINITY) {
+          const float w = __builtin_amdgcn_exp2f(x[i].x - M);
+          den = fmaf(w, x[i].y, den);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) num[j] = fmaf(w, v[i][j], num[j]);
+        }
     }
-    float mb = M;
+  if constexpr (PG > 1) {
+    sm[lr][pg][c] = M;
+    sd[lr][pg][c] = den;
+    so[lr][pg][c] = num;
+    __syncthreads();
+    if (pg != 0) return;
+    float all = M;
 #pragma unroll
-    for (int i = 0; i < kB; ++i) mb = fmaxf(mb, x[i].x);
-    const float alpha = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
-    M = mb;
-    den *= alpha;
-    num *= alpha;
+    for (int i = 1; i < PG; ++i) all = fmaxf(all, sm[lr][i][c]);
+    den = 0.0f;
+    num = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kB; ++i)
-      if (x[i].x != -INFINITY) {
-        const float w = __builtin_amdgcn_exp2f(x[i].x - M);
-        den = fmaf(w, x[i].y, den);
+    for (int i = 0; i < PG; ++i) {
+      const float m = sm[lr][i][c];
+      const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - all);
+      den = fmaf(w, sd[lr][i][c], den);
+      const f32x4 v = so[lr][i][c];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) num[j] = fmaf(w, v[i][j], num[j]);
-      }
+      for (int j = 0; j < 4; ++j) num[j] = fmaf(w, v[j], num[j]);
+    }
   }
+  if (!ok) return;
   const float inv = den > 0.0f ? 1.0f / den : den;
   struct alignas(4 * sizeof(Q)) Q4v {
     Q v[4];
@@ -832,27 +882,33 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
 
 struct Plan {
   int64_t shared_tiles, own_tiles;  // row tiles (own: an upper bound)
-  int shared_tile, shared_splits, shared_keys, own_splits, parts;
+  int shared_tile, shared_splits, own_from, own_splits, parts;
 };
 
-// Ranges: enough workgroups to give every compute unit two, and no range below 128 keys.
-int splits_for(int64_t items, int64_t keys) {
-  const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(items, 1));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, (keys + 127) / 128, 64})));
-}
+constexpr int kMaxSplits = 64;
 
 Plan plan_for(int64_t T, int g, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
   Plan p{};
   const int64_t rows = T * g;
-  // of ragged rows: at most one tile that is not full a sequence, and a full one has 64 rows at least (of 129 .. 192 rows: three tiles)
+  // The shared keys are a range of their own where that saves reading them once for each sequence: not for one sequence, not
+  // for a few keys, and not where a sequence's rows alone fill tiles (prompts), which then read them as often either
+  // way and need no join.
+  const bool apart = shared_len >= kTurn && batch > 1 && rows / batch < 128;
+  p.own_from = apart ? shared_len : 0;
+  // of ragged rows: at most one tile that is not full a sequence, and a full one has 64 rows at least (of 129 .. 192 rows:
+  // three tiles)
   p.own_tiles = ragged ? rows / 64 + batch : batch * static_cast<int64_t>(tiles_of(rows / batch, split));
-  p.own_splits = L > shared_len ? splits_for(n_kv * p.own_tiles, L - shared_len) : 0;
-  if (shared_len > 0) {
+  if (const int64_t keys = L - p.own_from; keys > 0) {
+    // Two workgroups for every compute unit, and no more: a workgroup's start and end are 4 to 5 us of dependent loads.
+    const int64_t items = n_kv * p.own_tiles;
+    p.own_splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({512 / items, (keys + kTurn - 1) / kTurn, kMaxSplits})));
+  }
+  if (apart) {
     p.shared_tile = tile_rows(rows, split);
     p.shared_tiles = tiles_of(rows, split);
-    const int s = splits_for(n_kv * p.shared_tiles, shared_len);
-    p.shared_keys = ((shared_len + s - 1) / s + kStage - 1) / kStage * kStage;
-    p.shared_splits = (shared_len + p.shared_keys - 1) / p.shared_keys;
+    p.shared_splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>({256 / (n_kv * p.shared_tiles), (shared_len + kTurn - 1) / kTurn, kMaxSplits})));
   }
   p.parts = p.shared_splits + p.own_splits;
   return p;
@@ -873,8 +929,11 @@ template <int QT, int CT, int HD>
 int launch(const AttnArgs& a, int64_t blocks, hipStream_t st) {
   hipLaunchKernelGGL((paged_attn_kernel<QT, CT, HD>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
   if (a.parts > 1) {
-    const int64_t threads = static_cast<int64_t>(a.T) * a.n_q * (HD / 4);
-    hipLaunchKernelGGL((paged_join_kernel<QT, HD>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, st, a);
+    // a few ranges a thread, so that a row is one round trip
+    const int64_t rows = static_cast<int64_t>(a.T) * a.n_q;
+    const auto fn = a.parts <= 4 ? paged_join_kernel<QT, HD, 1> : a.parts <= 16 ? paged_join_kernel<QT, HD, 4> : paged_join_kernel<QT, HD, 8>;
+    const int per = 256 / (HD / 4 * (a.parts <= 4 ? 1 : a.parts <= 16 ? 4 : 8));
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st, a);
   }
   return launch_status();
 }
@@ -931,9 +990,9 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
   a.o = a.ml + ml_floats(n);
   a.shared_pages = shared_pages;
   a.T = static_cast<int>(T), a.n_q = n_q, a.n_kv = kv->n_kv, a.g = g, a.L = L, a.shared_len = shared_len;
-  a.shared_blocks = static_cast<int>(shared_blocks), a.shared_splits = p.shared_splits, a.shared_keys = p.shared_keys;
+  a.shared_blocks = static_cast<int>(shared_blocks), a.shared_splits = p.shared_splits;
   a.shared_tile = p.shared_tile;
-  a.own_splits = p.own_splits, a.parts = p.parts;
+  a.own_from = p.own_from, a.own_splits = p.own_splits, a.parts = p.parts;
   // a negative scale turns q around and a zero one clears it, so that the exponents' factor is positive
   a.sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
   a.cs = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.44269504088896340736f;
