@@ -362,7 +362,7 @@ int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int b
  * accuracy (q and the softmax weights run as two fp16 terms; |q| < 65504), the others round the
  * weights to their own type. Sums, maxima and partial results are fp32; the result does not depend on timing. q_row and
  * q_head: elements between rows and heads, q and the strides multiples of 16 bytes, caches and out
- * 16-byte aligned. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or 128, 0 < L, 0 <= shared_len <= L,
+ * 16-byte aligned. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or 128, 0 < L <= 2^30, 0 <= shared_len <= L,
  * a finite scale, shared_len <= num_pages * page_size. Keys at or past L are not read. */
 int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, int64_t q_head, void* out, int dtype, int64_t T,
                int n_q, int L, const int32_t* shared_pages, int shared_len, float scale, void* workspace,

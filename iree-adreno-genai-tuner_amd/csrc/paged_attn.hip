@@ -58,13 +58,18 @@ struct AttnArgs {
   int64_t qr, qh;
   const void *kc, *vc;
   void* out;
-  float *ml, *o;  // ranges' (m, l) and o of each row: [T * n_q][parts]
+  // Results of ranges, (m, l) and o: first the shared ones, [T * n_q][shared_splits], then the slots of own ranges, slot_rows
+  // rows each. own: of each row the place of its first own range and their number.
+  float *ml, *o;
+  int2* own;  // null: every row has one range
   const int32_t* shared_pages;
   int T, n_q, n_kv, g, L, shared_len;
   int shared_blocks, shared_splits, shared_tile;  // workgroups of the shared ranges, ranges, rows of a workgroup
-  int own_from, own_splits, parts;                // own ranges: their first key, how many at most
+  int own_from, slot_rows;                        // own ranges: their first key, rows of a slot
+  bool longest_first;
   float cs, sign;  // exponents are s * cs in log2 units; sign: that of the scale, taken into q
-  FastDiv by_g, by_kv, by_shared, by_own;
+  int own_whole, own_items, own_most;             // items with all of their keys, items, ranges of an item at most
+  FastDiv by_g, by_kv, by_shared, by_ranges, by_tiles;
 };
 
 // Rows (token, head of the group) of a workgroup where there are `rows` in all. Up to 32 rows are not enough to share the
@@ -101,19 +106,66 @@ __host__ __device__ __forceinline__ int tiles_of(int64_t rows, bool split) {
   return static_cast<int>((rows + h - 1) / h);
 }
 
-// The sequence and, within it, the row tile of own tile `tile` (wave-uniform); false: past the last.
-__device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, bool split, int* seq, int* in_seq) {
-  if (!a.b.cu) {
-    const int per = tiles_of(static_cast<int64_t>(a.b.rows) * a.g, split);
-    *seq = tile / per;
-    *in_seq = tile - *seq * per;
-    return *seq < a.b.batch;
-  }
+constexpr int kMaxKeys = 1 << 30;  // positions of the blocks ahead stay below 2^31
+constexpr int kSlots = 512;    // own ranges at once: two workgroups on every compute unit
+constexpr int kMaxSplits = 64;  // ranges of a tile's keys
+
+// Own items are the tiles of each KV head. As many as fill the compute units whole times take all of their keys at once; the
+// rest, which would hold a few units and leave the others waiting, is split over all of them (of few items: all).
+struct Own {
+  int seq, tile, h;          // sequence, row tile in it, KV head
+  int range, ranges, slot0;  // ranges: at most; slot0: that of the item's first range (a single range has one beside
+                             // shared ranges only: without them it is the result)
+};
+
+// Item and range of own workgroup `idx` (wave-uniform); false: none.
+__device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split, Own* w) {
   const int lane = threadIdx.x & 63;
+  auto count = [&](int i) {  // lane: tiles of sequence i + lane
+    const int s = min(i + lane, a.b.batch - 1);
+    return i + lane < a.b.batch ? tiles_of(static_cast<int64_t>(tokens_of(a.b, s, a.T).y) * a.g, split) : 0;
+  };
+  int whole = a.own_whole, items = a.own_items;
+  FastDiv by_ranges = a.by_ranges;
+  if (a.b.cu) {
+    int tiles = 0;
+    for (int i = 0; i < a.b.batch; i += 64) tiles += count(i);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) tiles += __shfl_xor(tiles, m, 64);
+    items = __builtin_amdgcn_readfirstlane(tiles) * a.n_kv;
+    whole = items / kSlots * kSlots;
+    by_ranges.d = min(kSlots / max(items - whole, 1), a.own_most);
+  }
+  int item = idx;
+  w->range = 0, w->ranges = 1, w->slot0 = idx;
+  if (idx >= whole) {
+    w->ranges = by_ranges.d;
+    const int i = a.b.cu ? (idx - whole) / w->ranges : by_ranges.div(idx - whole);
+    w->range = idx - whole - i * w->ranges;
+    w->slot0 = (a.shared_splits ? whole : 0) + i * w->ranges;
+    item = whole + i;
+    if (item >= items) return false;
+  }
+  const int tile = a.by_kv.div(item);
+  w->h = item - tile * a.n_kv;
+  if (!a.b.cu) {
+    int s = a.by_tiles.div(tile);
+    w->tile = tile - s * a.by_tiles.d;
+    if (a.longest_first) {  // (a batch of 64 at most) the s-th longest
+      const int len = lane < a.b.batch ? a.b.lens[lane] : INT32_MIN;
+      int rank = 0;
+      for (int l = 0; l < a.b.batch; ++l) {
+        const int o = __builtin_amdgcn_readlane(len, l);
+        rank += o > len || (o == len && l < lane);
+      }
+      s = __builtin_ctzll(__ballot(lane < a.b.batch && rank == s));
+    }
+    w->seq = s;
+    return true;
+  }
   int base = 0;
   for (int i = 0; i < a.b.batch; i += 64) {
-    const int s = min(i + lane, a.b.batch - 1);
-    const int n = i + lane < a.b.batch ? tiles_of(static_cast<int64_t>(tokens_of(a.b, s, a.T).y) * a.g, split) : 0;
+    const int n = count(i);
     int run = n;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -123,8 +175,8 @@ __device__ __forceinline__ bool own_tile(const AttnArgs& a, int tile, bool split
     const uint64_t past = __ballot(base + run > tile);
     if (past) {
       const int l = __builtin_ctzll(past);
-      *seq = i + l;
-      *in_seq = tile - base - (__builtin_amdgcn_readlane(run, l) - __builtin_amdgcn_readlane(n, l));
+      w->seq = i + l;
+      w->tile = tile - base - (__builtin_amdgcn_readlane(run, l) - __builtin_amdgcn_readlane(n, l));
       return true;
     }
     base += __builtin_amdgcn_readlane(run, 63);
@@ -161,7 +213,8 @@ __device__ __forceinline__ const unsigned char* row_at(const unsigned char* base
 // keys, and their page entries, are known before the length of the sequence is.
 struct Item {
   bool shared;
-  int h, seq, row0, n_rows, tok0, part;  // rows row0 .. of the n_rows that start at token tok0
+  int h, seq, row0, n_rows, tok0;        // rows row0 .. of the n_rows that start at token tok0
+  int part, ranges, slot0;               // the range's number, how many there are, their first slot (own ranges)
   int k0, step, k1;                      // blocks at k0, k0 + step, .. below k1
   int own_end;                           // the keys of the sequence (own ranges)
   const int32_t* table;                  // its row of the page table
@@ -176,7 +229,7 @@ __device__ __forceinline__ int page_at(const AttnArgs& a, const Item& it, int j)
 
 // One row: its token and head, and how many keys of the range's kind it sees (0: none, or no row). Wave-uniform flow.
 struct Row {
-  int token, head, lim;
+  int token, head, lim, in_tile;
   bool ok;
 };
 __device__ __forceinline__ Row row_of(const AttnArgs& a, const Item& it, int r) {
@@ -186,6 +239,7 @@ __device__ __forceinline__ Row row_of(const AttnArgs& a, const Item& it, int r) 
   w.token = it.tok0 + i;
   w.head = it.h * a.g + r - i * a.g;
   w.lim = 0;
+  w.in_tile = r - it.row0;
   if (it.shared) {
     const int s = sequence_of_lane(a.b, w.ok ? w.token : 0);
     if (w.ok && s < a.b.batch) {
@@ -269,13 +323,15 @@ __device__ __forceinline__ void weights8(const float (&p)[8], float neg1, vec8<C
   }
 }
 
-// N consecutive values of a range's o (or, with one range, of the result) of a row.
+// N consecutive values of a range's o; or of the result, where it is the only range of the row.
 template <int QT, int HD, int N>
-__device__ __forceinline__ void store_o(const AttnArgs& a, const Row& w, int part, int d, const float (&v)[N], float m,
+__device__ __forceinline__ void store_o(const AttnArgs& a, const Item& it, const Row& w, int d, const float (&v)[N], float m,
                                         float l) {
   typedef typename Num<QT>::type Q;
-  const int64_t row = static_cast<int64_t>(w.token) * a.n_q + w.head;
-  if (a.parts == 1) {
+  const int64_t row = static_cast<int64_t>(w.token) * a.n_q + w.head, shared = static_cast<int64_t>(a.T) * a.n_q * a.shared_splits;
+  const int64_t first = shared + static_cast<int64_t>(it.slot0) * a.slot_rows + w.in_tile;
+  if (a.own && d == 0 && !it.shared && it.part == 0) a.own[row] = make_int2(static_cast<int>(first - shared), it.ranges);
+  if (!it.shared && it.ranges == 1 && a.shared_splits == 0) {
     const float inv = l > 0.0f ? 1.0f / l : l;  // no keys: zeros; NaN stays
     struct alignas(N * sizeof(Q) < 16 ? N * sizeof(Q) : 16) V {
       Q v[N];
@@ -284,7 +340,7 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Row& w, int par
     for (int i = 0; i < N; ++i) y.v[i] = static_cast<Q>(v[i] * inv);
     *reinterpret_cast<V*>(static_cast<Q*>(a.out) + row * HD + d) = y;
   } else {
-    const int64_t i = row * a.parts + part;
+    const int64_t i = it.shared ? row * a.shared_splits + it.part : first + static_cast<int64_t>(it.part) * a.slot_rows;
 #pragma unroll
     for (int j = 0; j < N; j += 4)
       *reinterpret_cast<f32x4*>(a.o + i * HD + d + j) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
@@ -485,7 +541,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     for (int e = threadIdx.x; e < 16 * kC4; e += kThreads) {
       const int r = e / kC4, c = e % kC4;
       Row y;
-      y.token = __shfl(w[x].token, r, 64), y.head = __shfl(w[x].head, r, 64);
+      y.token = __shfl(w[x].token, r, 64), y.head = __shfl(w[x].head, r, 64), y.in_tile = 16 * x + r;
       if (!__shfl(static_cast<int>(w[x].ok), r, 64)) continue;
       float mm = wml[0][16 * x + r].x;
 #pragma unroll
@@ -499,7 +555,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
         v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf_of(i)) + (16 * x + r) * HD + 4 * (c ^ r));
       }
       const float y4[4] = {v[0], v[1], v[2], v[3]};
-      store_o<QT, HD, 4>(a, y, it.part, 4 * c, y4, mm, den);
+      store_o<QT, HD, 4>(a, it, y, 4 * c, y4, mm, den);
     }
 }
 
@@ -742,7 +798,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
         v[i] = __builtin_bit_cast(float, lo);
         v[4 + i] = __builtin_bit_cast(float, hi);
       }
-      if (w.ok) store_o<QT, HD, 8>(a, w, it.part, 32 * d + 8 * (b + half), v, m, l);
+      if (w.ok) store_o<QT, HD, 8>(a, it, w, 32 * d + 8 * (b + half), v, m, l);
     }
 }
 
@@ -754,17 +810,24 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
   Item it;
   it.shared = idx < a.shared_blocks;
   if (!it.shared) idx -= a.shared_blocks;
-  const int hs = a.by_kv.div(idx);
-  it.h = idx - hs * a.n_kv;
-  int tile = it.shared ? a.by_shared.div(hs) : a.by_own.div(hs), height;
-  const int split = hs - tile * (it.shared ? a.shared_splits : a.own_splits);
-  it.seq = 0, it.tok0 = 0, it.own_end = 0, it.behind = 0, it.table = a.b.table;
+  int tile, height, split;
+  it.seq = 0, it.tok0 = 0, it.own_end = 0, it.behind = 0, it.table = a.b.table, it.slot0 = 0;
   if (it.shared) {
+    const int hs = a.by_kv.div(idx);
+    it.h = idx - hs * a.n_kv;
+    tile = a.by_shared.div(hs);
+    split = hs - tile * a.shared_splits;
+    it.ranges = a.shared_splits;
     height = a.shared_tile;
     it.n_rows = a.T * a.g;
   } else {
-    if (!own_tile(a, tile, QT == Q4_F32, &it.seq, &tile)) return;
-    it.seq = __builtin_amdgcn_readfirstlane(it.seq);
+    Own w;
+    if (!own_item(a, idx, QT == Q4_F32, &w)) return;
+    it.h = __builtin_amdgcn_readfirstlane(w.h);
+    it.seq = __builtin_amdgcn_readfirstlane(w.seq);
+    it.ranges = w.ranges, it.slot0 = w.slot0;
+    tile = __builtin_amdgcn_readfirstlane(w.tile);
+    split = w.range;
     const int2 tk = tokens_of(a.b, it.seq, a.T);
     it.tok0 = tk.x;
     it.n_rows = tk.y * a.g;
@@ -777,23 +840,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
   it.k0 = (it.shared ? 0 : a.own_from) + split * turn;
   const int first = it.k0 + (stream ? threadIdx.x >> 6 << 5 | (threadIdx.x & 31) : threadIdx.x & 63);
   const int entry = page_at(a, it, it.shared ? min(first, a.shared_len - 1) : max(first, 0));
-  if (it.shared) {
-    it.step = a.shared_splits * turn;
-    it.k1 = a.shared_len;
-    it.part = split;
-  } else {
+  it.part = split;
+  it.k1 = a.shared_len;
+  if (!it.shared) {
     const int len = a.b.lens[it.seq], tokens = a.b.cu ? it.n_rows / a.g : a.b.rows;
     it.own_end = min(a.b.keys_of(len), a.L);
     it.behind = len - tokens;
     // no row of the tile sees more than its last
     const int last = a.by_g.div(min(it.row0 + height, it.n_rows) - 1);
     it.k1 = min(it.own_end, it.behind + last + 1);
-    const int n = it.own_end - a.own_from;
-    const int ranges = min(a.own_splits, max((n + kTurn - 1) / kTurn, 1));
-    it.step = ranges * turn;
-    if (split >= ranges) it.k1 = it.k0;
-    it.part = a.shared_splits + split;
+    // no range without a block for every wave
+    it.ranges = min(it.ranges, max((it.k1 - a.own_from + kTurn - 1) / kTurn, 1));
+    if (split >= it.ranges) return;
   }
+  it.step = it.ranges * turn;
   if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, entry, buf0, buf1, wml);
   if constexpr (QT != Q4_F32)
     if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, entry, buf0, buf1, wml);
@@ -810,26 +870,34 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
   __shared__ float sm[kRowsWg][PG][kC4], sd[kRowsWg][PG][kC4];
   __shared__ f32x4 so[kRowsWg][PG][kC4];
   const int lr = threadIdx.x / kRow, pg = threadIdx.x % kRow / kC4, c = threadIdx.x % kC4;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsWg + lr;
-  bool ok = row < static_cast<int64_t>(a.T) * a.n_q;
+  const int64_t rows = static_cast<int64_t>(a.T) * a.n_q, row = static_cast<int64_t>(blockIdx.x) * kRowsWg + lr;
+  bool ok = row < rows;
   if (a.b.cu) {
     const int64_t t = row / a.n_q;
     ok = ok && t >= a.b.cu[0] && t < a.b.cu[a.b.batch];  // else of no sequence
   }
-  const float2* ml = reinterpret_cast<const float2*>(a.ml) + row * a.parts;
-  const float* o = a.o + row * a.parts * HD + 4 * c;
+  int2 own = make_int2(0, 0);
+  if (ok && a.L > a.own_from) own = a.own[row];
+  if (a.shared_splits == 0 && own.y == 1) ok = false;  // its one range has written the result
+  const int parts = a.shared_splits + own.y;
+  auto place = [&](int p) {
+    return p < a.shared_splits ? row * a.shared_splits + p
+                               : rows * a.shared_splits + own.x + static_cast<int64_t>(p - a.shared_splits) * a.slot_rows;
+  };
+  const float2* ml = reinterpret_cast<const float2*>(a.ml);
   float M = -INFINITY, den = 0.0f;
   f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
   if (ok)
-    for (int p0 = pg; p0 < a.parts; p0 += kB * PG) {
+    for (int p0 = pg; p0 < parts; p0 += kB * PG) {
       float2 x[kB];
       f32x4 v[kB];
 #pragma unroll
       for (int i = 0; i < kB; ++i) {
         x[i] = make_float2(-INFINITY, 0.0f);
-        if (p0 + i * PG < a.parts) {
-          x[i] = ml[p0 + i * PG];
-          v[i] = *reinterpret_cast<const f32x4*>(o + static_cast<int64_t>(p0 + i * PG) * HD);
+        if (p0 + i * PG < parts) {
+          const int64_t at = place(p0 + i * PG);
+          x[i] = ml[at];
+          v[i] = *reinterpret_cast<const f32x4*>(a.o + at * HD + 4 * c);
         }
       }
       float mb = M;
@@ -881,44 +949,65 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
 }
 
 struct Plan {
-  int64_t shared_tiles, own_tiles;  // row tiles (own: an upper bound)
-  int shared_tile, shared_splits, own_from, own_splits, parts;
+  int64_t shared_blocks, own_blocks;  // workgroups (own: an upper bound)
+  int64_t partials;                   // results of ranges that the workspace holds (0: none is needed)
+  int shared_tile, shared_splits, own_from, slot_rows;
+  int own_whole, own_items, own_ranges, own_most, own_tiles;  // (without cu_q) tiles of a sequence
+  int most;                                                    // ranges of a row at most
+  bool longest_first;
 };
 
-constexpr int kMaxSplits = 64;
-
-Plan plan_for(int64_t T, int g, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
+Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
   Plan p{};
+  const int g = n_q / n_kv;
   const int64_t rows = T * g;
   // The shared keys are a range of their own where that saves reading them once for each sequence: not for one sequence, not
   // for a few keys, and not where a sequence's rows alone fill tiles (prompts), which then read them as often either
   // way and need no join.
   const bool apart = shared_len >= kTurn && batch > 1 && rows / batch < 128;
   p.own_from = apart ? shared_len : 0;
-  // of ragged rows: at most one tile that is not full a sequence, and a full one has 64 rows at least (of 129 .. 192 rows:
-  // three tiles)
-  p.own_tiles = ragged ? rows / 64 + batch : batch * static_cast<int64_t>(tiles_of(rows / batch, split));
-  if (const int64_t keys = L - p.own_from; keys > 0) {
-    // Two workgroups for every compute unit, and no more: a workgroup's start and end are 4 to 5 us of dependent loads.
-    const int64_t items = n_kv * p.own_tiles;
-    p.own_splits = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({512 / items, (keys + kTurn - 1) / kTurn, kMaxSplits})));
-  }
   if (apart) {
+    // One workgroup for every compute unit: the other place of each is left to own ranges, and what ranges write and the join
+    // reads stays small (of 48 x 5 tokens x 32 heads and 4096 shared keys, 17 MB; with two 73 us, with one 62).
     p.shared_tile = tile_rows(rows, split);
-    p.shared_tiles = tiles_of(rows, split);
+    const int64_t items = n_kv * static_cast<int64_t>(tiles_of(rows, split));
     p.shared_splits = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>({256 / (n_kv * p.shared_tiles), (shared_len + kTurn - 1) / kTurn, kMaxSplits})));
+        1, std::min<int64_t>({kSlots / 2 / items, (shared_len + kTurn - 1) / kTurn, kMaxSplits})));
+    p.shared_blocks = items * p.shared_splits;
   }
-  p.parts = p.shared_splits + p.own_splits;
+  if (const int64_t keys = L - p.own_from; keys > 0) {
+    p.own_most = static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
+    if (ragged) {
+      // the number of tiles, and so of ranges, is known on the device alone; at most one tile that is not full a sequence, and
+      // a full one has 64 rows at least (of 129 .. 192 rows: three tiles)
+      p.own_blocks = (rows / 64 + batch) * n_kv + kSlots;
+      p.slot_rows = rows > 64 ? 128 : tile_rows(rows, split);
+    } else {
+      p.own_tiles = tiles_of(rows / batch, split);
+      const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv, rest = items % kSlots;
+      p.own_ranges = rest ? static_cast<int>(std::min<int64_t>(kSlots / rest, p.own_most)) : 1;
+      p.own_items = static_cast<int>(items), p.own_whole = static_cast<int>(items - rest);
+      p.own_blocks = items - rest + rest * p.own_ranges;
+      p.own_most = p.own_ranges;
+      p.slot_rows = tile_rows(rows / batch, split);
+    }
+    p.longest_first = !ragged && batch > 1 && batch <= 64 && keys > 4 * kTurn;
+  }
+  p.most = p.shared_splits + p.own_most;
+  if (p.most > 1) p.partials = T * n_q * p.shared_splits + p.slot_rows * (apart ? p.own_blocks : std::min<int64_t>(p.own_blocks, kSlots));
   return p;
 }
 
 size_t ml_floats(size_t n) { return (2 * n + 3) / 4 * 4; }
+size_t workspace_of(const Plan& p, int64_t rows, int hd) {
+  const size_t n = static_cast<size_t>(p.partials);
+  return n ? (ml_floats(n) + n * hd) * sizeof(float) + rows * sizeof(int2) : 0;
+}
 
 int attn_args(int64_t T, int n_q, int n_kv, int hd, int batch, int L, int shared_len) {
   if (T < 0 || T > INT32_MAX || n_q <= 0 || n_kv <= 0 || batch <= 0 || L <= 0 || shared_len < 0 || shared_len > L)
     return Q4_ERR_SHAPE;
+  if (L > kMaxKeys) return Q4_ERR_RANGE;
   if (n_q % n_kv || T * n_q > INT32_MAX) return Q4_ERR_SHAPE;
   if (hd != 64 && hd != 128) return Q4_ERR_UNSUPPORTED;
   if (n_q / n_kv > 64) return Q4_ERR_UNSUPPORTED;
@@ -926,13 +1015,14 @@ int attn_args(int64_t T, int n_q, int n_kv, int hd, int batch, int L, int shared
 }
 
 template <int QT, int CT, int HD>
-int launch(const AttnArgs& a, int64_t blocks, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attn_kernel<QT, CT, HD>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
-  if (a.parts > 1) {
-    // a few ranges a thread, so that a row is one round trip
+int launch(const AttnArgs& a, int64_t blocks, int most, hipStream_t st) {
+  if (blocks > 0)
+    hipLaunchKernelGGL((paged_attn_kernel<QT, CT, HD>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
+  if (most > 1) {
+    // a few ranges a thread, so that a row is one round trip; a thread a row where there are rows enough to fill the chip
     const int64_t rows = static_cast<int64_t>(a.T) * a.n_q;
-    const auto fn = a.parts <= 4 ? paged_join_kernel<QT, HD, 1> : a.parts <= 16 ? paged_join_kernel<QT, HD, 4> : paged_join_kernel<QT, HD, 8>;
-    const int per = 256 / (HD / 4 * (a.parts <= 4 ? 1 : a.parts <= 16 ? 4 : 8));
+    const int pg = most <= 4 || rows >= 16384 ? 1 : most <= 16 ? 4 : 8, per = 256 / (HD / 4 * pg);
+    const auto fn = pg == 1 ? paged_join_kernel<QT, HD, 1> : pg == 4 ? paged_join_kernel<QT, HD, 4> : paged_join_kernel<QT, HD, 8>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st, a);
   }
   return launch_status();
@@ -951,9 +1041,7 @@ extern "C" int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head
   for (const int form : {0, 1, 2, 3}) {  // cu_q or not, fp32 or not
     const bool ragged = form & 1, split = form & 2;
     if (!ragged && T % batch) continue;
-    const Plan p = plan_for(T, n_q / n_kv, n_kv, batch, ragged, split, L, shared_len);
-    const size_t n = static_cast<size_t>(T) * n_q * p.parts;
-    if (p.parts > 1) most = std::max(most, (ml_floats(n) + n * head_dim) * sizeof(float));
+    most = std::max(most, workspace_of(plan_for(T, n_q, n_kv, batch, ragged, split, L, shared_len), T * n_q, head_dim));
   }
   *bytes = most;
   return Q4_OK;
@@ -975,32 +1063,34 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     return Q4_ERR_ALIGN;
   if (T == 0) return Q4_OK;
   const int g = n_q / kv->n_kv;
-  const Plan p = plan_for(T, g, kv->n_kv, kv->batch, kv->cu_q != nullptr, dtype == Q4_F32, L, shared_len);
-  const size_t n = static_cast<size_t>(T) * n_q * p.parts;
-  if (p.parts > 1) {
-    if (!workspace || workspace_bytes < (ml_floats(n) + n * hd) * sizeof(float)) return Q4_ERR_WORKSPACE;
+  const Plan p = plan_for(T, n_q, kv->n_kv, kv->batch, kv->cu_q != nullptr, dtype == Q4_F32, L, shared_len);
+  if (p.partials) {
+    if (!workspace || workspace_bytes < workspace_of(p, T * n_q, hd)) return Q4_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return Q4_ERR_ALIGN;
   }
-  const int64_t shared_blocks = p.shared_tiles * p.shared_splits * kv->n_kv;
-  const int64_t blocks = shared_blocks + p.own_tiles * p.own_splits * kv->n_kv;
+  const int64_t blocks = p.shared_blocks + p.own_blocks;
   if (blocks > INT32_MAX) return Q4_ERR_SHAPE;
   a.q = q, a.qr = q_row, a.qh = q_head;
   a.kc = kv->k_cache, a.vc = kv->v_cache, a.out = out;
-  a.ml = static_cast<float*>(workspace);
-  a.o = a.ml + ml_floats(n);
+  if (p.partials) {
+    a.ml = static_cast<float*>(workspace);
+    a.o = a.ml + ml_floats(p.partials);
+    a.own = reinterpret_cast<int2*>(a.o + p.partials * hd);
+  }
   a.shared_pages = shared_pages;
   a.T = static_cast<int>(T), a.n_q = n_q, a.n_kv = kv->n_kv, a.g = g, a.L = L, a.shared_len = shared_len;
-  a.shared_blocks = static_cast<int>(shared_blocks), a.shared_splits = p.shared_splits;
-  a.shared_tile = p.shared_tile;
-  a.own_from = p.own_from, a.own_splits = p.own_splits, a.parts = p.parts;
+  a.shared_blocks = static_cast<int>(p.shared_blocks), a.shared_splits = p.shared_splits, a.shared_tile = p.shared_tile;
+  a.own_from = p.own_from, a.slot_rows = p.slot_rows, a.longest_first = p.longest_first;
   // a negative scale turns q around and a zero one clears it, so that the exponents' factor is positive
   a.sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
   a.cs = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.44269504088896340736f;
   a.by_g = FastDiv(g), a.by_kv = FastDiv(kv->n_kv);
-  a.by_shared = FastDiv(std::max(p.shared_splits, 1)), a.by_own = FastDiv(std::max(p.own_splits, 1));
+  a.own_whole = p.own_whole, a.own_items = p.own_items, a.own_most = p.own_most;
+  a.by_shared = FastDiv(std::max(p.shared_splits, 1)), a.by_ranges = FastDiv(std::max(p.own_ranges, 1));
+  a.by_tiles = FastDiv(std::max(p.own_tiles, 1));
   const hipStream_t st = as_stream(stream);
   const auto fn = dtype == Q4_F32    ? (hd == 128 ? launch<Q4_F32, Q4_F16, 128> : launch<Q4_F32, Q4_F16, 64>)
                   : dtype == Q4_F16  ? (hd == 128 ? launch<Q4_F16, Q4_F16, 128> : launch<Q4_F16, Q4_F16, 64>)
                                      : (hd == 128 ? launch<Q4_BF16, Q4_BF16, 128> : launch<Q4_BF16, Q4_BF16, 64>);
-  return fn(a, blocks, st);
+  return fn(a, blocks, p.most, st);
 }

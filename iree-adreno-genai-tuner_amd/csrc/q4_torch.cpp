@@ -372,7 +372,7 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (shared < 0 || shared > INT32_MAX || (shared > 0 && (!sp.defined() || sp.dim() != 1 || !indices(sp, sp.size(0), q) ||
                                                             sp.size(0) * p.kv.page_size < shared)))
       Py_RETURN_NONE;
-    if (a[9] == Py_None) L = std::min<int64_t>(std::max<int64_t>(int64_t{p.kv.max_pages} * p.kv.page_size, shared), INT32_MAX);
+    if (a[9] == Py_None) L = std::min<int64_t>(std::max<int64_t>(int64_t{p.kv.max_pages} * p.kv.page_size, shared), int64_t{1} << 30);
     else if (!arg(a[9], &L) || L < 1 || L > INT32_MAX) Py_RETURN_NONE;
     if (out.defined() && (!plain_as(out, dt) || out.dim() != 2 || out.size(0) != t || out.size(1) != n_q * hd || !same_device(out, q)))
       Py_RETURN_NONE;

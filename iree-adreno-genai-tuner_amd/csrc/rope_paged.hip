@@ -222,11 +222,11 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
       b = sequence_of(a.b, t);
       if (b < a.b.batch) {
         const int c0 = a.b.cu[b], c1 = a.b.cu[b + 1];
-        if (t >= c0 && c0 >= 0) p = a.b.lens[b] - c1 + t;
+        if (t >= c0 && c0 >= 0 && a.b.lens[b] >= 0) p = a.b.lens[b] - c1 + t;
       }
     } else {
       b = a.b.by_rows.div(t);
-      p = a.b.lens[b] - a.b.rows + (t - b * a.b.rows);
+      if (a.b.lens[b] >= 0) p = a.b.lens[b] - a.b.rows + (t - b * a.b.rows);
     }
     if (p >= 0) {
       const int page = a.b.by_page.div(p);

@@ -593,7 +593,7 @@ def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shar
     if q.stride(0) % align or q.stride(1) % align or q.data_ptr() % 16:
         q = q.contiguous()
     if L is None:
-        L = min(max(kv.max_pages * kv.page_size, shared_len), (1 << 31) - 1)
+        L = min(max(kv.max_pages * kv.page_size, shared_len), 1 << 30)
     need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len)
     if workspace is None:
         workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)

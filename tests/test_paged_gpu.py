@@ -352,6 +352,21 @@ def test_paged_attn_ragged_tails(dev, n, n_q, n_kv):
     b.check(q, 0.125, workspace=ws)
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("n,rows,lens,shared,n_kv", [(70, 1, 150, 130, 8), (140, 1, 40, 0, 4), (3, 130, 400, 0, 64),
+                                                     (3, 130, 500, 300, 64), (2, 300, 310, 0, 48)])
+def test_paged_attn_more_tiles_than_places(dev, dt, ragged, n, rows, lens, shared, n_kv):
+    """More tiles of rows and heads than the chip takes at once: those past whole rounds are split over it. The workspace is
+    full of NaN, and a second call with other queries on it is right too."""
+    r = [rows - (i % 2 if rows > 1 else 0) if ragged else rows for i in range(n)]
+    b = Batch(dev, dt, 64, n_kv, 16, [lens + 5 * (i % 7) for i in range(n)], r, shared, ragged, seed=n)
+    L = b.page_table.shape[1] * 16
+    ws = torch.full((ops.paged_attn_workspace_bytes(b.tokens, n_kv, n_kv, 64, n, L, shared),), 255, dtype=torch.uint8, device=dev)
+    for _ in range(2):
+        b.check(b.q(n_kv), 0.125, workspace=ws if ws.numel() else None)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 0.01, 2.0])
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 def test_paged_attn_scales(dev, dt, scale):
