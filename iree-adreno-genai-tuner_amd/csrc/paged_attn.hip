@@ -68,7 +68,7 @@ struct AttnArgs {
   int own_from, slot_rows;                        // own ranges: their first key, rows of a slot
   bool longest_first;
   float cs, sign;  // exponents are s * cs in log2 units; sign: that of the scale, taken into q
-  int own_whole, own_items, own_most;             // items with all of their keys, items, ranges of an item at most
+  int own_whole, own_items, own_most, places;     // items with all of their keys, items, ranges of an item at most and of all
   FastDiv by_g, by_kv, by_shared, by_ranges, by_tiles;
 };
 
@@ -79,7 +79,7 @@ struct AttnArgs {
 __host__ __device__ __forceinline__ int tile_rows(int64_t rows, bool split) {
   if (rows <= 16) return 16;
   if (rows <= 32 && !split) return 32;
-  return rows <= 64 || (rows > 128 && rows <= 192) ? 64 : 128;
+  return rows <= 64 ? 64 : 128;
 }
 
 // The sequence of token t, another in each lane (batch or more: none). Every lane of the wave takes part.
@@ -134,7 +134,7 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split,
     for (int m = 32; m >= 1; m >>= 1) tiles += __shfl_xor(tiles, m, 64);
     items = __builtin_amdgcn_readfirstlane(tiles) * a.n_kv;
     whole = items / kSlots * kSlots;
-    by_ranges.d = min(kSlots / max(items - whole, 1), a.own_most);
+    by_ranges.d = max(min(a.places / max(items - whole, 1), a.own_most), 1);
   }
   int item = idx;
   w->range = 0, w->ranges = 1, w->slot0 = idx;
@@ -952,7 +952,7 @@ struct Plan {
   int64_t shared_blocks, own_blocks;  // workgroups (own: an upper bound)
   int64_t partials;                   // results of ranges that the workspace holds (0: none is needed)
   int shared_tile, shared_splits, own_from, slot_rows;
-  int own_whole, own_items, own_ranges, own_most, own_tiles;  // (without cu_q) tiles of a sequence
+  int places, own_whole, own_items, own_ranges, own_most, own_tiles;  // (without cu_q) tiles of a sequence
   int most;                                                    // ranges of a row at most
   bool longest_first;
 };
@@ -975,17 +975,18 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, 
         1, std::min<int64_t>({kSlots / 2 / items, (shared_len + kTurn - 1) / kTurn, kMaxSplits})));
     p.shared_blocks = items * p.shared_splits;
   }
+  p.places = kSlots - static_cast<int>(std::min<int64_t>(p.shared_blocks, kSlots / 2));  // what shared ranges leave
   if (const int64_t keys = L - p.own_from; keys > 0) {
     p.own_most = static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
     if (ragged) {
       // the number of tiles, and so of ranges, is known on the device alone; at most one tile that is not full a sequence, and
-      // a full one has 64 rows at least (of 129 .. 192 rows: three tiles)
-      p.own_blocks = (rows / 64 + batch) * n_kv + kSlots;
-      p.slot_rows = rows > 64 ? 128 : tile_rows(rows, split);
+      // a full one has 128 rows
+      p.own_blocks = (rows / 128 + batch) * n_kv + kSlots;
+      p.slot_rows = tile_rows(rows, split);
     } else {
       p.own_tiles = tiles_of(rows / batch, split);
       const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv, rest = items % kSlots;
-      p.own_ranges = rest ? static_cast<int>(std::min<int64_t>(kSlots / rest, p.own_most)) : 1;
+      p.own_ranges = rest ? static_cast<int>(std::max<int64_t>(std::min<int64_t>(p.places / rest, p.own_most), 1)) : 1;
       p.own_items = static_cast<int>(items), p.own_whole = static_cast<int>(items - rest);
       p.own_blocks = items - rest + rest * p.own_ranges;
       p.own_most = p.own_ranges;
@@ -1085,7 +1086,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
   a.sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
   a.cs = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.44269504088896340736f;
   a.by_g = FastDiv(g), a.by_kv = FastDiv(kv->n_kv);
-  a.own_whole = p.own_whole, a.own_items = p.own_items, a.own_most = p.own_most;
+  a.own_whole = p.own_whole, a.own_items = p.own_items, a.own_most = p.own_most, a.places = p.places;
   a.by_shared = FastDiv(std::max(p.shared_splits, 1)), a.by_ranges = FastDiv(std::max(p.own_ranges, 1));
   a.by_tiles = FastDiv(std::max(p.own_tiles, 1));
   const hipStream_t st = as_stream(stream);
