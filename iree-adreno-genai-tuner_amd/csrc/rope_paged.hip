@@ -13,19 +13,49 @@
 #include "q4_paged.h"
 
 #include <algorithm>
+#include <initializer_list>
+
+// Which product of a sum is fused is written out: left to the compiler it differs between the kernels of one operator, and
+// a token's result would depend on how many are rotated with it.
+#pragma clang fp contract(off)
 
 namespace q4 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kU = 4;  // units in flight per thread
+constexpr int kU = 2;  // units in flight per thread (8192 tokens of 40 heads of 128, bf16: 40.7 us with 4, 38.2 with 2)
+
+// Calls past this many bytes (the L2s together) go around the caches: nothing of them would be found there again, and
+// what they displace would. 8192 tokens of 40 heads of 128, bf16: 38.2 -> 32 us, which is the time of a copy; with nothing
+// to save (a few tokens) the rotated q stays in the cache for the attention that follows.
+constexpr int64_t kStream = 32 << 20;
+
+// V at p, around the caches if NT and V is a whole 16 bytes.
+template <bool NT, typename V>
+__device__ __forceinline__ V load_v(const void* p) {
+  if constexpr (NT && sizeof(V) == 16) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(V, __builtin_nontemporal_load(static_cast<const u32x4*>(p)));
+  } else {
+    return *static_cast<const V*>(p);
+  }
+}
+template <bool NT, typename V>
+__device__ __forceinline__ void store_v(void* p, const V& v) {
+  if constexpr (NT && sizeof(V) == 16) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), static_cast<u32x4*>(p));
+  } else {
+    *static_cast<V*>(p) = v;
+  }
+}
 
 // One unit of a head: a pair of vectors (half layout, rotated part), or one vector of interleaved pairs or of the
-// part that is not rotated. E elements per vector; E == 1: pairs of elements, then single ones.
-template <int DT, int LAYOUT, bool VEC>
+// part that is not rotated. Vectors of VB bytes (16 or 8); VB == 0: pairs of elements, then single ones.
+template <int DT, int LAYOUT, int VB>
 struct Unit {
   typedef typename Num<DT>::type T;
-  static constexpr int E = VEC ? 16 / sizeof(T) : 1;
+  static constexpr int E = VB ? VB / static_cast<int>(sizeof(T)) : 1;
   struct alignas(E * sizeof(T)) V {
     T v[E];
   };
@@ -34,34 +64,35 @@ struct Unit {
   // Element offsets of a unit's vectors in its head (second: -1 for none).
   static __device__ __forceinline__ int first(int u, int half) {
     if constexpr (LAYOUT == Q4_ROPE_HALF) return u < half / E ? u * E : 2 * half + (u - half / E) * E;
-    return VEC ? u * E : 2 * u;
+    return VB ? u * E : 2 * u;
   }
   static __device__ __forceinline__ int second(int u, int half) {
     if constexpr (LAYOUT == Q4_ROPE_HALF) return u < half / E ? half + u * E : -1;
-    return VEC ? -1 : 2 * u + 1;
+    return VB ? -1 : 2 * u + 1;
   }
   // Units of a head of hd dims; those of its rotated part alone.
-  static int count(int hd, int half) { return LAYOUT == Q4_ROPE_HALF ? half / E + (hd - 2 * half) / E : VEC ? hd / E : hd / 2; }
-  static int rotated(int half) { return LAYOUT == Q4_ROPE_HALF ? half / E : VEC ? (2 * half + E - 1) / E : half; }
+  static int count(int hd, int half) { return LAYOUT == Q4_ROPE_HALF ? half / E + (hd - 2 * half) / E : VB ? hd / E : hd / 2; }
+  static int rotated(int half) { return LAYOUT == Q4_ROPE_HALF ? half / E : VB ? (2 * half + E - 1) / E : half; }
 
+  template <bool NT>
   __device__ __forceinline__ void load(const T* head, int u, int half) {
-    a = *reinterpret_cast<const V*>(head + first(u, half));
+    a = load_v<NT, V>(head + first(u, half));
     const int s = second(u, half);
-    if (s >= 0) b = *reinterpret_cast<const V*>(head + s);
+    if (s >= 0) b = load_v<NT, V>(head + s);
   }
   // Rotates by the token's table of (cos, sin); pairs past `half` keep their values.
   __device__ __forceinline__ void rotate(const float2* cs, int u, int half) {
     auto pair = [&](T& x, T& y, int i) {
       const float2 w = cs[i];
       const float p = static_cast<float>(x), q = static_cast<float>(y);
-      x = static_cast<T>(p * w.x - q * w.y);
-      y = static_cast<T>(q * w.x + p * w.y);
+      x = static_cast<T>(fmaf(p, w.x, -(q * w.y)));
+      y = static_cast<T>(fmaf(q, w.x, p * w.y));
     };
     if constexpr (LAYOUT == Q4_ROPE_HALF) {
       if (u < half / E)
 #pragma unroll
         for (int e = 0; e < E; ++e) pair(a.v[e], b.v[e], u * E + e);
-    } else if constexpr (VEC) {
+    } else if constexpr (VB != 0) {
 #pragma unroll
       for (int e = 0; e < E / 2; ++e)
         if (u * (E / 2) + e < half) pair(a.v[2 * e], a.v[2 * e + 1], u * (E / 2) + e);
@@ -69,7 +100,7 @@ struct Unit {
       pair(a.v[0], b.v[0], u);
     }
   }
-  template <typename C>
+  template <bool NT, typename C>
   __device__ __forceinline__ void store(C* head, int u, int half) const {
     struct alignas(E * sizeof(C)) W {
       C v[E];
@@ -78,7 +109,7 @@ struct Unit {
       W w;
 #pragma unroll
       for (int e = 0; e < E; ++e) w.v[e] = static_cast<C>(x.v[e]);
-      *reinterpret_cast<W*>(head + off) = w;
+      store_v<NT>(head + off, w);
     };
     put(a, first(u, half));
     const int s = second(u, half);
@@ -112,12 +143,12 @@ __device__ __forceinline__ void fill_tables(float2* cs, const int* pos, int n, c
 }
 
 // x, y: T tokens of H heads; workgroup (x, y): tokens x * tpb .., part y of their units.
-template <int DT, int LAYOUT, bool VEC>
+template <int DT, int LAYOUT, int VB, bool NT>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const void* x_, int64_t xr, int64_t xh, void* y_, int64_t yr,
                                                        int64_t yh, int T, int tpb, int H, int units, int part,
                                                        const int32_t* __restrict__ positions, RopeArgs r, FastDiv by_units,
                                                        FastDiv by_heads, FastDiv by_half) {
-  typedef Unit<DT, LAYOUT, VEC> U;
+  typedef Unit<DT, LAYOUT, VB> U;
   typedef typename U::T E;
   extern __shared__ float2 lds[];
   int* pos = reinterpret_cast<int*>(lds);
@@ -134,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const void* x_, int64_t 
       const int i = base + k * kThreads;
       if (i < end) {
         const int hh = by_units.div(i), t = by_heads.div(hh);
-        w[k].load(x + (t0 + t) * xr + (hh - t * H) * xh, i - hh * units, r.half);
+        w[k].template load<NT>(x + (t0 + t) * xr + (hh - t * H) * xh, i - hh * units, r.half);
       }
     }
   };
@@ -151,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const void* x_, int64_t 
       if (i < end) {
         const int hh = by_units.div(i), t = by_heads.div(hh), u = i - hh * units;
         w[k].rotate(cs + t * r.half, u, r.half);
-        w[k].store(y + (t0 + t) * yr + (hh - t * H) * yh, u, r.half);
+        w[k].template store<NT>(y + (t0 + t) * yr + (hh - t * H) * yh, u, r.half);
       }
     }
   }
@@ -178,9 +209,9 @@ __device__ __forceinline__ int sequence_of(const PagedBatch& b, int t) {
   return n;
 }
 
-template <int DT, int CT, int LAYOUT, bool VEC>
+template <int DT, int CT, int LAYOUT, int VB, bool NT>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
-  typedef Unit<DT, LAYOUT, VEC> U;
+  typedef Unit<DT, LAYOUT, VB> U;
   typedef typename U::T E;
   typedef typename Num<CT>::type C;
   extern __shared__ float2 lds[];
@@ -209,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
         const E* p = h < a.n_kv       ? static_cast<const E*>(a.k) + tt * a.kr + h * a.kh
                      : h < 2 * a.n_kv ? static_cast<const E*>(a.v) + tt * a.vr + (h - a.n_kv) * a.vh
                                       : static_cast<const E*>(a.q) + tt * a.qr + (h - 2 * a.n_kv) * a.qh;
-        w[k].load(p, u, half);
+        w[k].template load<NT>(p, u, half);
       }
     }
   };
@@ -251,10 +282,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
         const int64_t s = slot[t];
         if (h < a.n_kv || h >= 2 * a.n_kv) w[k].rotate(cs + t * half, u, half);
         if (h >= 2 * a.n_kv) {
-          if (pos[t] >= 0) w[k].store(static_cast<E*>(a.qo) + (t0 + t) * a.por + (h - 2 * a.n_kv) * a.poh, u, half);
+          if (pos[t] >= 0) w[k].template store<NT>(static_cast<E*>(a.qo) + (t0 + t) * a.por + (h - 2 * a.n_kv) * a.poh, u, half);
         } else if (s >= 0) {
           C* c = static_cast<C*>(h < a.n_kv ? a.kc : a.vc);
-          w[k].store(c + (s * a.n_kv + (h < a.n_kv ? h : h - a.n_kv)) * a.hd, u, half);
+          w[k].template store<NT>(c + (s * a.n_kv + (h < a.n_kv ? h : h - a.n_kv)) * a.hd, u, half);
         }
       }
     }
@@ -277,8 +308,6 @@ Split split_for(int64_t T, int per_token, int half) {
   return s;
 }
 
-bool whole(int64_t n, int e) { return n % e == 0; }
-
 int rope_args(const q4_rope* rope, int hd, RopeArgs* r, int* layout) {
   *r = RopeArgs{nullptr, 0, 1.0f, 1.0f};
   *layout = Q4_ROPE_HALF;
@@ -294,39 +323,33 @@ int rope_args(const q4_rope* rope, int hd, RopeArgs* r, int* layout) {
 
 size_t bytes_of(int dt) { return dt == Q4_F32 ? 4 : 2; }
 
-// Whether heads of hd dims with `half` rotated pairs are whole 16-byte vectors (the interleaved layout needs
-// no boundary between its rotated pairs and the rest on a vector).
-bool whole_heads(int hd, int half, int layout, int e) {
-  return whole(hd, e) && (layout == Q4_ROPE_INTERLEAVED || whole(half, e));
-}
-
-template <int DT, int LAYOUT, bool VEC>
+template <int DT, int LAYOUT, int VB>
 int launch_rope(const void* x, int64_t xr, int64_t xh, void* y, int64_t yr, int64_t yh, int64_t T, int heads, int hd,
                 const int32_t* positions, const RopeArgs& r, hipStream_t st) {
-  typedef Unit<DT, LAYOUT, VEC> U;
+  typedef Unit<DT, LAYOUT, VB> U;
   const bool in_place = x == y && xr == yr && xh == yh;
   const int units = in_place ? U::rotated(r.half) : U::count(hd, r.half);
   if (units == 0) return Q4_OK;
   const Split s = split_for(T, heads * units, r.half);
   const size_t lds = 8 * ((s.tpb + 1) / 2 + static_cast<size_t>(s.tpb) * r.half);
-  hipLaunchKernelGGL((rope_kernel<DT, LAYOUT, VEC>), dim3(static_cast<unsigned>((T + s.tpb - 1) / s.tpb), s.parts),
+  const bool stream = T * heads * hd * static_cast<int64_t>(sizeof(typename U::T)) > kStream;
+  const auto fn = VB == 16 && stream ? rope_kernel<DT, LAYOUT, VB, VB == 16> : rope_kernel<DT, LAYOUT, VB, false>;
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((T + s.tpb - 1) / s.tpb), s.parts),
                      dim3(kThreads), lds, st, x, xr, xh, y, yr, yh, static_cast<int>(T), s.tpb, heads, units, s.part,
                      positions, r, FastDiv(units), FastDiv(heads), FastDiv(std::max(r.half, 1)));
   return launch_status();
 }
 
-template <int DT>
-int launch_rope1(bool vec, int layout, const void* x, int64_t xr, int64_t xh, void* y, int64_t yr, int64_t yh, int64_t T,
-                 int heads, int hd, const int32_t* positions, const RopeArgs& r, hipStream_t st) {
-  const auto fn = layout == Q4_ROPE_HALF ? (vec ? launch_rope<DT, Q4_ROPE_HALF, true> : launch_rope<DT, Q4_ROPE_HALF, false>)
-                                         : (vec ? launch_rope<DT, Q4_ROPE_INTERLEAVED, true>
-                                                : launch_rope<DT, Q4_ROPE_INTERLEAVED, false>);
+template <int DT, int LAYOUT>
+int launch_rope1(int vb, const void* x, int64_t xr, int64_t xh, void* y, int64_t yr, int64_t yh, int64_t T, int heads, int hd,
+                 const int32_t* positions, const RopeArgs& r, hipStream_t st) {
+  const auto fn = vb == 16 ? launch_rope<DT, LAYOUT, 16> : vb == 8 ? launch_rope<DT, LAYOUT, 8> : launch_rope<DT, LAYOUT, 0>;
   return fn(x, xr, xh, y, yr, yh, T, heads, hd, positions, r, st);
 }
 
-template <int DT, int CT, int LAYOUT, bool VEC>
+template <int DT, int CT, int LAYOUT, int VB>
 int launch_append(AppendArgs& a, hipStream_t st) {
-  a.units = Unit<DT, LAYOUT, VEC>::count(a.hd, a.r.half);
+  a.units = Unit<DT, LAYOUT, VB>::count(a.hd, a.r.half);
   const Split s = split_for(a.T, a.heads * a.units, a.r.half);
   a.tpb = s.tpb;
   a.part = s.part;
@@ -334,17 +357,35 @@ int launch_append(AppendArgs& a, hipStream_t st) {
   a.by_heads = FastDiv(a.heads);
   a.by_half = FastDiv(std::max(a.r.half, 1));
   const size_t lds = 8 * (s.tpb + static_cast<size_t>(s.tpb) * a.r.half);
-  hipLaunchKernelGGL((append_kernel<DT, CT, LAYOUT, VEC>), dim3((a.T + s.tpb - 1) / s.tpb, s.parts), dim3(kThreads), lds,
+  const bool stream = static_cast<int64_t>(a.T) * a.heads * a.hd * static_cast<int64_t>(sizeof(typename Num<DT>::type)) > kStream;
+  const auto fn = VB == 16 && stream ? append_kernel<DT, CT, LAYOUT, VB, VB == 16> : append_kernel<DT, CT, LAYOUT, VB, false>;
+  hipLaunchKernelGGL(fn, dim3((a.T + s.tpb - 1) / s.tpb, s.parts), dim3(kThreads), lds,
                      st, a);
   return launch_status();
 }
 
 template <int DT, int CT>
-int launch_append1(bool vec, int layout, AppendArgs& a, hipStream_t st) {
-  if (layout == Q4_ROPE_HALF)
-    return vec ? launch_append<DT, CT, Q4_ROPE_HALF, true>(a, st) : launch_append<DT, CT, Q4_ROPE_HALF, false>(a, st);
-  return vec ? launch_append<DT, CT, Q4_ROPE_INTERLEAVED, true>(a, st)
-             : launch_append<DT, CT, Q4_ROPE_INTERLEAVED, false>(a, st);
+int launch_append1(int vb, int layout, AppendArgs& a, hipStream_t st) {
+  const bool half = layout == Q4_ROPE_HALF;
+  const auto fn = vb == 16  ? (half ? launch_append<DT, CT, Q4_ROPE_HALF, 16> : launch_append<DT, CT, Q4_ROPE_INTERLEAVED, 16>)
+                  : vb == 8 ? (half ? launch_append<DT, CT, Q4_ROPE_HALF, 8> : launch_append<DT, CT, Q4_ROPE_INTERLEAVED, 8>)
+                            : (half ? launch_append<DT, CT, Q4_ROPE_HALF, 0> : launch_append<DT, CT, Q4_ROPE_INTERLEAVED, 0>);
+  return fn(a, st);
+}
+
+// The widest vectors, in bytes, in which heads of hd dims with `half` rotated pairs, operands at these addresses and these
+// strides are whole (the interleaved layout needs no boundary between its rotated pairs and the rest on a vector);
+// 0: none. Odd halves and starts go element by element (8192 tokens of 40 heads, 62 of 128 dims rotated by halves: 74 us).
+int vector_bytes(int hd, int half, int layout, size_t es, std::initializer_list<const void*> at,
+                 std::initializer_list<int64_t> strides) {
+  for (const int vb : {16, 8}) {
+    const int e = vb / static_cast<int>(es);
+    bool ok = hd % e == 0 && (layout == Q4_ROPE_INTERLEAVED || half % e == 0);
+    for (const void* p : at) ok = ok && aligned(p, vb);
+    for (const int64_t s : strides) ok = ok && s % e == 0;
+    if (ok) return vb;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -368,11 +409,12 @@ extern "C" int rope_rotate(const void* x, int64_t x_row, int64_t x_head, void* y
   if (!aligned(x, es) || !aligned(y, es) || !aligned(positions, 4)) return Q4_ERR_ALIGN;
   if (T == 0) return Q4_OK;
   r.sign = inverse ? -1.0f : 1.0f;
-  const int e = static_cast<int>(16 / es);
-  const bool vec = aligned(x, 16) && aligned(y, 16) && whole_heads(head_dim, r.half, layout, e) && whole(x_row, e) &&
-                   whole(x_head, e) && whole(y_row, e) && whole(y_head, e);
-  const auto fn = dtype == Q4_F32 ? launch_rope1<Q4_F32> : dtype == Q4_F16 ? launch_rope1<Q4_F16> : launch_rope1<Q4_BF16>;
-  return fn(vec, layout, x, x_row, x_head, y, y_row, y_head, T, heads, head_dim, positions, r, as_stream(stream));
+  const int vb = vector_bytes(head_dim, r.half, layout, es, {x, y}, {x_row, x_head, y_row, y_head});
+  const bool half = layout == Q4_ROPE_HALF;
+  const auto fn = dtype == Q4_F32   ? (half ? launch_rope1<Q4_F32, Q4_ROPE_HALF> : launch_rope1<Q4_F32, Q4_ROPE_INTERLEAVED>)
+                  : dtype == Q4_F16 ? (half ? launch_rope1<Q4_F16, Q4_ROPE_HALF> : launch_rope1<Q4_F16, Q4_ROPE_INTERLEAVED>)
+                                    : (half ? launch_rope1<Q4_BF16, Q4_ROPE_HALF> : launch_rope1<Q4_BF16, Q4_ROPE_INTERLEAVED>);
+  return fn(vb, x, x_row, x_head, y, y_row, y_head, T, heads, head_dim, positions, r, as_stream(stream));
 }
 
 extern "C" int paged_kv_append(const q4_paged_kv* kv, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -394,14 +436,8 @@ extern "C" int paged_kv_append(const q4_paged_kv* kv, const void* k, int64_t k_r
       !aligned(kv->v_cache, cs))
     return Q4_ERR_ALIGN;
   if (T == 0) return Q4_OK;
-  const int e = static_cast<int>(16 / es);
-  bool vec = aligned(k, 16) && aligned(v, 16) && aligned(kv->k_cache, 16) && aligned(kv->v_cache, 16) &&
-             whole_heads(hd, a.r.half, layout, e);
-  for (int64_t s : {k_row, k_head, v_row, v_head}) vec = vec && whole(s, e);
-  if (q) {
-    vec = vec && aligned(q, 16) && aligned(q_out, 16);
-    for (int64_t s : {q_row, q_head, qo_row, qo_head}) vec = vec && whole(s, e);
-  }
+  const int vb = vector_bytes(hd, a.r.half, layout, es, {k, v, kv->k_cache, kv->v_cache, q, q_out},
+                              {k_row, k_head, v_row, v_head, q ? q_row : 0, q ? q_head : 0, q ? qo_row : 0, q ? qo_head : 0});
   a.k = k, a.kr = k_row, a.kh = k_head;
   a.v = v, a.vr = v_row, a.vh = v_head;
   a.q = q, a.qr = q_row, a.qh = q_head;
@@ -409,7 +445,7 @@ extern "C" int paged_kv_append(const q4_paged_kv* kv, const void* k, int64_t k_r
   a.kc = kv->k_cache, a.vc = kv->v_cache;
   a.T = static_cast<int>(T), a.n_kv = kv->n_kv, a.heads = static_cast<int>(heads), a.hd = hd;
   const hipStream_t st = as_stream(stream);
-  if (dtype == Q4_F32) return launch_append1<Q4_F32, Q4_F16>(vec, layout, a, st);
-  if (dtype == Q4_F16) return launch_append1<Q4_F16, Q4_F16>(vec, layout, a, st);
-  return launch_append1<Q4_BF16, Q4_BF16>(vec, layout, a, st);
+  if (dtype == Q4_F32) return launch_append1<Q4_F32, Q4_F16>(vb, layout, a, st);
+  if (dtype == Q4_F16) return launch_append1<Q4_F16, Q4_F16>(vb, layout, a, st);
+  return launch_append1<Q4_BF16, Q4_BF16>(vb, layout, a, st);
 }

@@ -72,7 +72,7 @@ def check_rounded(got, ref, err, dt):
 @pytest.mark.parametrize("interleaved", [False, True], ids=["half", "inter"])
 @pytest.mark.parametrize("t,h,hd,rot", [(1, 1, 2, 2), (1, 32, 128, 128), (7, 5, 64, 32), (33, 3, 80, 80), (5, 4, 80, 38),
                                         (3, 2, 96, 30), (2, 3, 256, 256), (1200, 9, 64, 64), (4, 2, 1024, 1024),
-                                        (3, 2, 10, 6), (6, 4, 64, 0)])
+                                        (3, 2, 10, 6), (6, 4, 64, 0), (9, 3, 80, 40), (9, 3, 100, 100)])
 def test_rope_rotate(dev, dt, interleaved, t, h, hd, rot):
     g = torch.Generator().manual_seed(t * 7 + hd)
     x = torch.randn(t, h, hd, generator=g).to(dt).to(dev)
@@ -87,6 +87,27 @@ def test_rope_rotate(dev, dt, interleaved, t, h, hd, rot):
     # in place: the same bits
     y = x.clone()
     assert ops.rope_rotate(y, pos, rope, out=y) is y and torch.equal(y, got)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_large_calls_go_around_the_caches_with_the_same_bits(dev, dt):
+    """Past 32 MB the loads and stores bypass the caches: what they give is what the same tokens give in small calls."""
+    t, n_q, n_kv, hd = (20000 if dt == torch.float32 else 40000), 4, 2, 64
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(t, n_q + 2 * n_kv, hd, generator=g).to(dt).to(dev)
+    pos = torch.arange(t, dtype=torch.int32, device=dev)
+    rope = Rope(freqs(hd, dev))
+    assert qkv.numel() * qkv.element_size() > 32 << 20
+    big = ops.rope_rotate(qkv, pos, rope)
+    assert all(torch.equal(ops.rope_rotate(qkv[i:i + 5000], pos[i:i + 5000], rope), big[i:i + 5000]) for i in range(0, t, 5000))
+    table = torch.randperm(t // 16, generator=g).int().to(dev)[None]
+    caches = [torch.zeros(t // 16, 16, n_kv, hd, dtype=cache_of(dt), device=dev) for _ in range(4)]
+    q = ops.paged_kv_append(qkv[:, n_q:n_q + n_kv], qkv[:, n_q + n_kv:], *caches[:2], table, i32([t], dev), rope=rope, q=qkv[:, :n_q])
+    assert torch.equal(q, big[:, :n_q])
+    for i in range(0, t, 5000):
+        s = qkv[i:i + 5000]
+        ops.paged_kv_append(s[:, n_q:n_q + n_kv], s[:, n_q + n_kv:], *caches[2:], table, i32([i + 5000], dev), rope=rope)
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
 
 
 def test_rope_far_and_negative_positions(dev):
@@ -251,7 +272,7 @@ APPENDS = [  # page, lens, rows, ragged
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 @pytest.mark.parametrize("page,lens,rows,ragged", APPENDS)
-@pytest.mark.parametrize("n_q,n_kv,hd,rot,inter", [(6, 2, 128, 128, False), (5, 5, 64, 32, True), (3, 1, 80, 38, False),
+@pytest.mark.parametrize("n_q,n_kv,hd,rot,inter", [(6, 2, 128, 128, False), (5, 5, 64, 32, True), (3, 1, 80, 38, False), (2, 3, 80, 40, False),
                                                    (2, 2, 64, None, False)])
 def test_paged_kv_append(dev, dt, page, lens, rows, ragged, n_q, n_kv, hd, rot, inter):
     b = Batch(dev, dt, hd, n_kv, page, lens, rows, ragged=ragged, seed=len(lens) + page, extra=2 if ragged else 0)
