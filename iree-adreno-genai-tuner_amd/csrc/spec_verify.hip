@@ -5,9 +5,9 @@
 // r sum(w). The product of two fp32 numbers is exact in fp64 and so is nearly every difference, and sums are
 // fp64 in a fixed order, so the choice is that of the definition but within about 1e-14 of a border.
 //
-// Two launches, each one pass: the first decides j (every workgroup for itself: two dependent round trips
-// instead of a launch) and sums w over chunks of kChunk values; the second finds the chunk by a scan of the chunk
-// sums, and reads that chunk again for the index. Only one row of p and one of q is read in full, whatever the number
+// Two launches, each one pass: the first decides j (every wave for itself: two dependent round trips instead of a
+// launch) and sums w over chunks of kChunk values, a wave each; the second finds the chunk by a scan of the chunk sums, and
+// reads that chunk again for the index. Only one row of p and one of q is read in full, whatever the number
 // of drafts. Bound: HBM for large batches, the dependent loads for one sequence.
 #include "q4_common.h"
 
@@ -17,8 +17,9 @@ namespace q4 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 4;                           // float4s per thread and row
-constexpr int kChunk = kThreads * 4 * kPer;       // values of a row per workgroup
+constexpr int kWaves = kThreads / 64;
+constexpr int kChunk = kThreads * 4;              // values of a row that are summed together: a wave's, and 4 a thread of the pick
+constexpr int kPer = kChunk / (64 * 4);           // float4s per lane of a wave that sums a chunk
 
 struct VerifyArgs {
   const int32_t* tokens;
@@ -96,35 +97,33 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// A wave sums a chunk: no barrier.
 __global__ __launch_bounds__(kThreads) void verify_sum_kernel(VerifyArgs a) {
-  const int b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
+  const int groups = (a.chunks + kWaves - 1) / kWaves;
+  const int b = blockIdx.x / groups, c = (blockIdx.x - b * groups) * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (c >= a.chunks) return;
   int drafted;
   const int j = accepted_of(a, b, &drafted);
   const Weights w = weights_of(a, b, j, drafted);
   float p[kPer][4], q[kPer][4] = {};
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) load4(w.p, c * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, p[k]);
+  for (int k = 0; k < kPer; ++k) load4(w.p, c * kChunk + (k * 64 + lane) * 4, a.V, p[k]);
   if (w.q) {
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) load4(w.q, c * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, q[k]);
+    for (int k = 0; k < kPer; ++k) load4(w.q, c * kChunk + (k * 64 + lane) * 4, a.V, q[k]);
   }
   double s = 0.0, sp = 0.0;
 #pragma unroll
   for (int k = 0; k < kPer; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s += weight(w, c * kChunk + (k * kThreads + threadIdx.x) * 4 + i, p[k][i], q[k][i]);
+      s += weight(w, c * kChunk + (k * 64 + lane) * 4 + i, p[k][i], q[k][i]);
       sp += positive(p[k][i]);
     }
   s = wave_sum(s);
   sp = wave_sum(sp);
-  __shared__ double2 part[kThreads / 64];
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_double2(s, sp);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double2 t = part[0];
-    for (int i = 1; i < kThreads / 64; ++i) t.x += part[i].x, t.y += part[i].y;
-    a.sums[blockIdx.x] = t;
+  if (lane == 0) {
+    a.sums[static_cast<int64_t>(b) * a.chunks + c] = make_double2(s, sp);
     if (c == 0) a.accepted[b] = j;
   }
 }
@@ -151,7 +150,7 @@ __device__ __forceinline__ void block_scan(double (&v)[N], double (*part)[N], do
   for (int k = 0; k < N; ++k) {
     double before = 0.0, all = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
       if (i == wave) before = all;
       all += part[i][k];
     }
@@ -170,20 +169,20 @@ __device__ __forceinline__ int2 block_min_max(int lo, int hi, int2* part) {
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_int2(lo, hi);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) lo = min(lo, part[i].x), hi = max(hi, part[i].y);
+  for (int i = 0; i < kWaves; ++i) lo = min(lo, part[i].x), hi = max(hi, part[i].y);
   return make_int2(lo, hi);
 }
 
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   const int b = blockIdx.x;
-  __shared__ double sums_s[kThreads / 64][2], in_s[kThreads / 64][kPer], before_s;
-  __shared__ int2 mm[2][kThreads / 64];
+  __shared__ double sums_s[kWaves][2], in_s[kWaves][1], before_s;
+  __shared__ int2 mm[2][kWaves];
   const int drafted = a.n_draft ? min(max(a.n_draft[b], 0), a.K) : a.K;
   const int j = a.accepted[b];
   const double u = a.uniforms[b * a.uni_row + a.K];
   const double2* sums = a.sums + static_cast<int64_t>(b) * a.chunks;
   auto load = [&](int c) { return c < a.chunks ? sums[c] : make_double2(0.0, 0.0); };
-  // the sums of all chunks; one tile of kThreads chunks (1 M values) is kept with its running sums
+  // the sums of all chunks; one tile of kThreads chunks (256 K values) is kept with its running sums
   const double2 mine = load(threadIdx.x);
   double run[2] = {mine.x, mine.y}, all[2];
   block_scan(run, sums_s, all);
@@ -207,7 +206,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
       s = f ? s2.y : s2.x;
       double v[1] = {s}, w[1];
       __syncthreads();
-      block_scan(v, reinterpret_cast<double(*)[1]>(&in_s[0][0]), w);
+      block_scan(v, in_s, w);
       r = carry + v[0];
       t = w[0];
     }
@@ -224,36 +223,24 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
   if (chunk >= 0) {
     Weights w = weights_of(a, b, j, drafted);
     if (f) w.q = nullptr, w.zero = -1;
-    float p[kPer][4], q[kPer][4] = {};
+    const int e = chunk * kChunk + threadIdx.x * 4;
+    float p[4], q[4] = {};
+    load4(w.p, e, a.V, p);
+    if (w.q) load4(w.q, e, a.V, q);
+    double v[4], s[1], t[1];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) load4(w.p, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, p[k]);
-    if (w.q) {
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) load4(w.q, chunk * kChunk + (k * kThreads + threadIdx.x) * 4, a.V, q[k]);
-    }
-    double s[kPer], t[kPer];
-    auto value = [&](int k, int i) { return weight(w, chunk * kChunk + (k * kThreads + threadIdx.x) * 4 + i, p[k][i], q[k][i]); };
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) s[k] = ((value(k, 0) + value(k, 1)) + value(k, 2)) + value(k, 3);
-    double own[kPer];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) own[k] = s[k];
+    for (int i = 0; i < 4; ++i) v[i] = weight(w, e + i, p[i], q[i]);
+    const double own = ((v[0] + v[1]) + v[2]) + v[3];
+    s[0] = own;
     block_scan(s, in_s, t);
-    double before = before_s;
+    double r = before_s + (s[0] - own);
     int lo = INT32_MAX, hi = -1;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      double r = before + (s[k] - own[k]);
-      before += t[k];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double v = value(k, i);
-        r += v;
-        const int e = chunk * kChunk + (k * kThreads + threadIdx.x) * 4 + i;
-        if (v > 0.0) {
-          if (r > limit) lo = min(lo, e);
-          hi = max(hi, e);
-        }
+    for (int i = 0; i < 4; ++i) {
+      r += v[i];
+      if (v[i] > 0.0) {
+        if (r > limit) lo = min(lo, e + i);
+        hi = max(hi, e + i);
       }
     }
     const int2 at = block_min_max(lo, hi, mm[1]);
@@ -294,7 +281,7 @@ extern "C" int spec_verify(const int32_t* tokens, int64_t tok_row, const float* 
   VerifyArgs a{tokens, draft, target, uniforms, n_draft, tok_row, draft_batch, draft_row, target_batch, target_row, uni_row,
                K, static_cast<int>(V), chunks_of(V), static_cast<double2*>(workspace), out_tokens, n_accepted};
   const hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(verify_sum_kernel, dim3(static_cast<unsigned>(B) * a.chunks), dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL(verify_sum_kernel, dim3(static_cast<unsigned>(B) * ((a.chunks + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
   hipLaunchKernelGGL(verify_pick_kernel, dim3(B), dim3(kThreads), 0, st, a);
   return launch_status();
 }
