@@ -360,10 +360,13 @@ int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int b
  * only: the shared keys are read and multiplied once for the whole batch. shared_len 0: shared_pages unused.
  * dtype (of q and out): F32 or F16 with an F16 cache, BF16 with a BF16 cache; F32 keeps fp32-level
  * accuracy (q and the softmax weights run as two fp16 terms; |q| < 65504), the others round the
- * weights to their own type. Sums, maxima and partial results are fp32; the result does not depend on timing. q_row and
+ * weights to their own type. Sums, maxima and partial results are fp32; the result does not depend on timing.
+ * Rows of the cache that hold no key of a sequence may hold anything; the values of keys 0 .. seq_lens - 1 and of the
+ * shared keys are finite, also those that a token does not see (a NaN there can reach tokens before it). q_row and
  * q_head: elements between rows and heads, q and the strides multiples of 16 bytes, caches and out
- * 16-byte aligned. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or 128, 0 < L <= 2^30, 0 <= shared_len <= L,
- * a finite scale, shared_len <= num_pages * page_size. Keys at or past L are not read. */
+ * 16-byte aligned; out overlaps neither q nor the caches. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or
+ * 128, 0 < L <= 2^30, 0 <= shared_len <= L, a finite scale, shared_len <= num_pages * page_size. Keys at or past L are
+ * not read. */
 int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, int64_t q_head, void* out, int dtype, int64_t T,
                int n_q, int L, const int32_t* shared_pages, int shared_len, float scale, void* workspace,
                size_t workspace_bytes, void* stream);

@@ -962,9 +962,11 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, 
   const int g = n_q / n_kv;
   const int64_t rows = T * g;
   // The shared keys are a range of their own where that saves reading them once for each sequence: not for one sequence, not
-  // for a few keys, and not where a sequence's rows alone fill tiles (prompts), which then read them as often either
-  // way and need no join.
-  const bool apart = shared_len >= kTurn && batch > 1 && rows / batch < 128;
+  // for a few keys (they cost their ranges' partial results and join), and not where a sequence's rows alone fill tiles
+  // (prompts), which then read them as often either way and need no join. One token each of 2 / 8 / 32 sequences, 32/8
+  // heads of 128, 200 own keys, apart and not: 256 shared keys 9.1 / 12.9 / 16.1 and 9.0 / 10.4 / 15.0 us, 1024 keys
+  // 9.5 / 13.8 / 17.2 and 9.8 / 15.0 / 23.5, 16384 keys 20.7 / 27.2 / 36.1 and 26.5 / 54.5 / 163.
+  const bool apart = shared_len >= 4 * kTurn && batch > 1 && rows / batch < 128;
   p.own_from = apart ? shared_len : 0;
   if (apart) {
     // One workgroup for every compute unit: the other place of each is left to own ranges, and what ranges write and the join
@@ -1070,7 +1072,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     if (!aligned(workspace, 16)) return Q4_ERR_ALIGN;
   }
   const int64_t blocks = p.shared_blocks + p.own_blocks;
-  if (blocks > INT32_MAX) return Q4_ERR_SHAPE;
+  if (blocks > INT32_MAX || p.partials > INT32_MAX) return Q4_ERR_SHAPE;
   a.q = q, a.qr = q_row, a.qh = q_head;
   a.kc = kv->k_cache, a.vc = kv->v_cache, a.out = out;
   if (p.partials) {

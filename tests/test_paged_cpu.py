@@ -80,9 +80,20 @@ def attend(kv=None, q=FAKE, row=256, head=64, out=FAKE, dt=F16, T=6, n_q=4, L=64
     (dict(kv=paged(head_dim=96)), "UNSUPPORTED"), (dict(n_q=130), "UNSUPPORTED"), (dict(scale=math.inf), "RANGE"),
     (dict(scale=math.nan), "RANGE"), (dict(kv=paged(num_pages=1), shared=33), "RANGE"), (dict(q=FAKE + 8), "ALIGN"),
     (dict(out=FAKE + 8), "ALIGN"), (dict(kv=paged(k_cache=FAKE + 8)), "ALIGN"), (dict(sp=FAKE + 1), "ALIGN"),
-    (dict(ws=FAKE + 8), "ALIGN"), (dict(ws=None), "WORKSPACE"), (dict(nbytes=64), "WORKSPACE")])
+    (dict(L=(1 << 30) + 1), "RANGE")])
 def test_paged_attn_refuses(bad, code):
     assert attend(**bad) == ERR[code]
+
+
+@pytest.mark.parametrize("bad,code", [(dict(ws=FAKE + 8), "ALIGN"), (dict(ws=None), "WORKSPACE"), (dict(nbytes=64), "WORKSPACE")])
+@pytest.mark.parametrize("shared", [0, 1024])
+def test_paged_attn_refuses_a_workspace(bad, code, shared):
+    """Where a row has several ranges of keys (one range writes the result itself and needs none)."""
+    big = dict(kv=paged(num_pages=1000, max_pages=256, table_stride=256), L=4096, shared=shared)
+    assert attend(**big, **bad) == ERR[code]
+    b = C.c_size_t(0)
+    assert LIB.raw("paged_attn_workspace_bytes")(6, 4, 2, 64, 3, 4096, shared, C.byref(b)) == 0 and b.value > 64
+    assert attend(**big, nbytes=64) == ERR["WORKSPACE"]
 
 
 def verify(tok=FAKE, draft=FAKE, target=FAKE, u=FAKE, nd=None, B=2, K=3, V=100, out=FAKE, acc=FAKE, ws=FAKE, nbytes=1 << 20,
@@ -203,3 +214,24 @@ def test_rope_params_part_of_a_head_and_unknown_types():
         rope_params({**CFG, "rope_scaling": {"rope_type": "other", "factor": 2.0}})
     with pytest.raises(NotImplementedError):
         inv_freq({**CFG, "rope_scaling": {"rope_type": "yarn", "factor": 2.0}})
+
+
+@pytest.mark.parametrize("bad", [None, 1, "x", torch.zeros(2, 4, dtype=torch.int32), torch.zeros(0), object()])
+def test_native_calls_leave_the_rest_to_python(bad):
+    """Anything but plain device tensors of the documented types: None, nothing raised, nothing launched."""
+    from q4llm._lib import native_calls
+    mod = native_calls()
+    x, pos, f, (k, v) = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32), torch.ones(32), caches()
+    ok = [x, pos, f, False, 1.0, False, None]
+    for i in range(7):
+        assert mod.rope(*ok[:i], bad, *ok[i + 1:]) is None
+    ok = [x, x, k, v, TABLE, LENS, None, f, False, 1.0, x, None]
+    for i in range(12):
+        assert mod.append(*ok[:i], bad, *ok[i + 1:]) is None
+    ok = [x, k, v, TABLE, LENS, 0.1, None, None, 0, None, None, None]
+    for i in range(12):
+        assert mod.paged(*ok[:i], bad, *ok[i + 1:]) is None
+    ok = [pos.view(1, 3), None, torch.zeros(1, 4, 9), torch.zeros(1, 4), None, None]
+    for i in range(6):
+        assert mod.verify(*ok[:i], bad, *ok[i + 1:]) is None
+    assert mod.rope() is None and mod.append(x) is None and mod.paged() is None and mod.verify() is None

@@ -355,6 +355,53 @@ def test_paged_attn(dev, dt, n_q, n_kv, hd, page, lens, rows, shared, ragged):
     assert (out[sum(rows):] == 9).all()  # tokens of no sequence
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("page,lens,rows,shared,ragged,n_q,n_kv,hd", [
+    (16, [600, 650, 520, 0, 300], [1] * 5, 520, False, 6, 2, 128),          # one tile of the streaming form, empty, shorter
+    (24, [700] * 9, [2] * 9, 640, False, 4, 2, 64),                          # 36 rows: two waves for the keys
+    (7, [560 + i for i in range(40)], [1 + i % 3 for i in range(40)], 513, True, 3, 1, 64),
+    (16, [900 + 9 * i for i in range(30)], [3] * 30, 800, False, 4, 1, 128),  # 360 rows: tiles of 128
+    (64, [1500, 1400, 1290], [60, 1, 20], 1281, True, 8, 2, 128),
+    (32, [515, 512, 100, 700], [4] * 4, 512, False, 4, 4, 128)])
+def test_paged_attn_prefix_as_a_range_of_its_own(dev, dt, page, lens, rows, shared, ragged, n_q, n_kv, hd):
+    b = Batch(dev, dt, hd, n_kv, page, lens, rows, shared, ragged, seed=shared, extra=2 if ragged else 0)
+    q = b.q(n_q)
+    out = torch.full((b.tokens, n_q * hd), 9.0, dtype=dt, device=dev)
+    L = max(b.page_table.shape[1] * page, shared)
+    ws = torch.full((ops.paged_attn_workspace_bytes(b.tokens, n_q, n_kv, hd, len(lens), L, shared),), 255, dtype=torch.uint8,
+                    device=dev)
+    b.check(q, hd ** -0.5, out=out, workspace=ws)
+    assert (out[sum(rows):] == 9).all()
+    # L at the prefix: no range of the sequences' own
+    b.check(q, hd ** -0.5, L=shared)
+
+
+def test_native_calls_and_python_wrappers_agree(dev, monkeypatch):
+    """The same bits whichever of the two checks the arguments."""
+    b = Batch(dev, torch.float16, 64, 2, 16, [200, 90, 150], [2, 2, 2], 64, seed=3)
+    qkv = torch.randn(6, 8, 64, generator=b.g).half().to(dev)
+    rope = Rope(freqs(64, dev), True, 1.25)
+    pos = torch.arange(6, dtype=torch.int32, device=dev)
+    tok, draft, target, u, _ = drafts(dev, 3, 2, 500, 4)
+    k0, v0 = b.k.clone(), b.v.clone()
+
+    def everything():
+        b.k.copy_(k0)
+        b.v.copy_(v0)
+        r = [ops.rope_rotate(qkv, pos, rope), ops.rope_rotate(qkv, pos, rope, inverse=True)]
+        r.append(ops.paged_kv_append(qkv[:, 4:6], qkv[:, 6:], b.k, b.v, b.page_table, b.seq_lens, rope=rope, q=qkv[:, :4]))
+        assert ops.paged_kv_append(qkv[:, 4:6], qkv[:, 6:], b.k, b.v, b.page_table, b.seq_lens, rope=rope) is None
+        r += [b.attn(r[-1], 0.125), b.attn(r[-1], 0.125, L=170), b.k.clone().view(torch.int16), b.v.clone().view(torch.int16)]
+        r += [*ops.spec_verify(tok, draft, target, u), *ops.spec_verify(tok, None, target, u, n_draft=i32([1, 0, 2], dev))]
+        return r
+
+    assert all(getattr(ops, n) is not ops._left_to_python for n in ("_rope", "_append", "_paged", "_verify"))
+    native = everything()
+    for n in ("_rope", "_append", "_paged", "_verify"):
+        monkeypatch.setattr(ops, n, ops._left_to_python)
+    assert all(torch.equal(x, y) for x, y in zip(native, everything()))
+
+
 @pytest.mark.parametrize("n_q,n_kv", [(64, 1), (20, 4), (7, 7), (48, 1)])
 def test_paged_attn_group_sizes(dev, n_q, n_kv):
     b = Batch(dev, torch.float16, 64, n_kv, 16, [70, 100], [2, 2], 48, seed=n_q)
@@ -362,20 +409,20 @@ def test_paged_attn_group_sizes(dev, n_q, n_kv):
 
 
 @pytest.mark.parametrize("n_q,n_kv", [(1, 1), (3, 1), (10, 2)])
-@pytest.mark.parametrize("n", [5, 17, 23, 40, 67, 129])
-def test_paged_attn_ragged_tails(dev, n, n_q, n_kv):
+@pytest.mark.parametrize("n,shared", [(5, 130), (17, 520), (23, 520), (40, 520), (67, 520), (129, 130), (129, 520)])
+def test_paged_attn_ragged_tails(dev, n, shared, n_q, n_kv):
     """Batches whose rows end inside a tile, the workspace full of NaN: every row of every range is written."""
     rows = [1 + (i * 7) % 3 for i in range(n)]
-    b = Batch(dev, torch.float16, 64, n_kv, 8, [150 + 3 * i for i in range(n)], rows, 130, True, seed=n, extra=1)
+    b = Batch(dev, torch.float16, 64, n_kv, 8, [shared + 20 + 3 * (i % 40) for i in range(n)], rows, shared, True, seed=n, extra=1)
     q = b.q(n_q)
     L = b.page_table.shape[1] * 8
-    ws = torch.full((ops.paged_attn_workspace_bytes(b.tokens, n_q, n_kv, 64, n, L, 130),), 255, dtype=torch.uint8, device=dev)
+    ws = torch.full((ops.paged_attn_workspace_bytes(b.tokens, n_q, n_kv, 64, n, L, shared),), 255, dtype=torch.uint8, device=dev)
     b.check(q, 0.125, workspace=ws)
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 @pytest.mark.parametrize("ragged", [False, True])
-@pytest.mark.parametrize("n,rows,lens,shared,n_kv", [(70, 1, 150, 130, 8), (140, 1, 40, 0, 4), (3, 130, 400, 0, 64),
+@pytest.mark.parametrize("n,rows,lens,shared,n_kv", [(70, 1, 540, 520, 8), (140, 1, 40, 0, 4), (3, 130, 400, 0, 64),
                                                      (3, 130, 500, 300, 64), (2, 300, 310, 0, 48)])
 def test_paged_attn_more_tiles_than_places(dev, dt, ragged, n, rows, lens, shared, n_kv):
     """More tiles of rows and heads than the chip takes at once: those past whole rounds are split over it. The workspace is
