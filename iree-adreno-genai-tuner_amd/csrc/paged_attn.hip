@@ -65,8 +65,9 @@ struct AttnArgs {
   const int32_t* shared_pages;
   int T, n_q, n_kv, g, L, shared_len;
   int shared_blocks, shared_splits, shared_tile;  // workgroups of the shared ranges, ranges, rows of a workgroup
-  int own_from, slot_rows;                        // own ranges: their first key, rows of a slot
-  bool longest_first;
+  int own_from, slot_rows, own_rows;              // own ranges: their first key, rows of a slot and of all slots
+  bool longest_first, refill;
+  int turn_from;
   float cs, sign;  // exponents are s * cs in log2 units; sign: that of the scale, taken into q
   int own_whole, own_items, own_most, places;     // items with all of their keys, items, ranges of an item at most and of all
   FastDiv by_g, by_kv, by_shared, by_ranges, by_tiles;
@@ -110,6 +111,17 @@ constexpr int kMaxKeys = 1 << 30;  // positions of the blocks ahead stay below 2
 constexpr int kSlots = 512;    // own ranges at once: two workgroups on every compute unit
 constexpr int kMaxSplits = 64;  // ranges of a tile's keys
 
+// Ranges of each of `items` that share `places`: as many as fit at once, or, where those leave more than an eighth of the
+// places free, as many as fill them twice (the last ones start as the first end; `refill`: not with tiles of the shared
+// form, whose ranges cost more to start: 10 prompts of 100 tokens 72 -> 76 us). One token each of 12 / 20 / 24 sequences of
+// 1000 to 6000 keys, 16 heads of 64: 49.7 / 79.9 / 86.3 -> 43.2 / 64.6 / 87.2 us; 8 KV heads of 128, 24 / 40 sequences:
+// 82 / 138 -> 74 / 115. Where they do fit (8 sequences of 16 heads), the second filling costs: 33.5 -> 34.7 us.
+__host__ __device__ __forceinline__ int ranges_of(int items, int places, bool refill, int most) {
+  int n = places / items;
+  if (refill && 8 * n * items < 7 * places) n = 2 * places / items;
+  return n < 1 ? 1 : n < most ? n : most;
+}
+
 // Own items are the tiles of each KV head. As many as fill the compute units whole times take all of their keys at once; the
 // rest, which would hold a few units and leave the others waiting, is split over all of them (of few items: all).
 struct Own {
@@ -134,7 +146,7 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split,
     for (int m = 32; m >= 1; m >>= 1) tiles += __shfl_xor(tiles, m, 64);
     items = __builtin_amdgcn_readfirstlane(tiles) * a.n_kv;
     whole = items / kSlots * kSlots;
-    by_ranges.d = max(min(a.places / max(items - whole, 1), a.own_most), 1);
+    by_ranges.d = ranges_of(max(items - whole, 1), a.places, a.refill, a.own_most);
   }
   int item = idx;
   w->range = 0, w->ranges = 1, w->slot0 = idx;
@@ -148,11 +160,14 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split,
   }
   const int tile = a.by_kv.div(item);
   w->h = item - tile * a.n_kv;
+  // Longest first (a batch of 64 at most): those that wait for a place are short. Where none waits and each compute unit gets a
+  // second one, the second ones go shortest first, so that the longest and the shortest share a unit.
+  const int len = lane < a.b.batch && a.longest_first ? a.b.lens[lane] : INT32_MIN;
   if (!a.b.cu) {
     int s = a.by_tiles.div(tile);
     w->tile = tile - s * a.by_tiles.d;
-    if (a.longest_first) {  // (a batch of 64 at most) the s-th longest
-      const int len = lane < a.b.batch ? a.b.lens[lane] : INT32_MIN;
+    if (a.longest_first) {  // the s-th longest
+      if (s >= a.turn_from) s = a.b.batch - 1 - (s - a.turn_from);
       int rank = 0;
       for (int l = 0; l < a.b.batch; ++l) {
         const int o = __builtin_amdgcn_readlane(len, l);
@@ -161,6 +176,25 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split,
       s = __builtin_ctzll(__ballot(lane < a.b.batch && rank == s));
     }
     w->seq = s;
+    return true;
+  }
+  if (a.longest_first) {  // lane: a sequence, its tiles from `before` on
+    const int n = count(0);
+    int before = 0;
+    for (int l = 0; l < a.b.batch; ++l) {
+      const int o = __builtin_amdgcn_readlane(len, l), t = __builtin_amdgcn_readlane(n, l);
+      before += o > len || (o == len && l < lane) ? t : 0;
+    }
+    if (a.shared_blocks == 0 && whole == 0 && items * w->ranges <= kSlots) {
+      const bool second = before * a.n_kv * w->ranges >= kSlots / 2;
+      int firsts = 0;
+      for (uint64_t m = __ballot(!second && n > 0); m; m &= m - 1) firsts += __builtin_amdgcn_readlane(n, __builtin_ctzll(m));
+      if (second) before = firsts + a.by_kv.div(items) - before - n;
+    }
+    const uint64_t here = __ballot(before <= tile && tile < before + n);
+    if (!here) return false;
+    w->seq = __builtin_ctzll(here);
+    w->tile = tile - __builtin_amdgcn_readlane(before, w->seq);
     return true;
   }
   int base = 0;
@@ -879,6 +913,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
   int2 own = make_int2(0, 0);
   if (ok && a.L > a.own_from) own = a.own[row];
   if (a.shared_splits == 0 && own.y == 1) ok = false;  // its one range has written the result
+  // (where cu_q does not ascend, a row may have no range, and `own` anything)
+  if (own.x < 0 || own.y < 0 || own.y > kMaxSplits || own.x >= a.own_rows - (own.y - 1) * a.slot_rows) own.y = 0;
   const int parts = a.shared_splits + own.y;
   auto place = [&](int p) {
     return p < a.shared_splits ? row * a.shared_splits + p
@@ -954,7 +990,8 @@ struct Plan {
   int shared_tile, shared_splits, own_from, slot_rows;
   int places, own_whole, own_items, own_ranges, own_most, own_tiles;  // (without cu_q) tiles of a sequence
   int most;                                                    // ranges of a row at most
-  bool longest_first;
+  int turn_from;  // the second ones: sequences from here on
+  bool longest_first, refill;
 };
 
 Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
@@ -979,25 +1016,37 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, 
   }
   p.places = kSlots - static_cast<int>(std::min<int64_t>(p.shared_blocks, kSlots / 2));  // what shared ranges leave
   if (const int64_t keys = L - p.own_from; keys > 0) {
+    p.refill = rows / batch <= 32;  // (of sequences of different lengths: the mean)
+    const int slots = p.refill ? 2 * kSlots : kSlots;
     p.own_most = static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
     if (ragged) {
       // the number of tiles, and so of ranges, is known on the device alone; at most one tile that is not full a sequence, and
       // a full one has 128 rows
-      p.own_blocks = (rows / 128 + batch) * n_kv + kSlots;
+      p.own_blocks = (rows / 128 + batch) * n_kv + slots;
       p.slot_rows = tile_rows(rows, split);
     } else {
       p.own_tiles = tiles_of(rows / batch, split);
       const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv, rest = items % kSlots;
-      p.own_ranges = rest ? static_cast<int>(std::max<int64_t>(std::min<int64_t>(p.places / rest, p.own_most), 1)) : 1;
+      p.own_ranges = rest ? ranges_of(static_cast<int>(rest), p.places, p.refill, p.own_most) : 1;
       p.own_items = static_cast<int>(items), p.own_whole = static_cast<int>(items - rest);
       p.own_blocks = items - rest + rest * p.own_ranges;
       p.own_most = p.own_ranges;
       p.slot_rows = tile_rows(rows / batch, split);
     }
-    p.longest_first = !ragged && batch > 1 && batch <= 64 && keys > 4 * kTurn;
+    // One token each of 8 / 16 / 28 sequences of 1000 to 6000 keys, 16 heads of 64, the second ones longest first too and
+    // shortest first: 36.0 / 63.2 / 105 and 32.9 / 55.7 / 90 us. Up to three tokens each, 8 KV heads of 128, in the batch's order
+    // and so: 38.6 / 64.5 / 109 and 34.8 / 58.0 / 93.
+    p.longest_first = batch > 1 && batch <= 64 && keys > 4 * kTurn;
+    p.turn_from = batch;
+    if (!apart && !ragged && p.own_blocks <= kSlots) {
+      const int64_t each = p.own_blocks / batch;
+      p.turn_from = static_cast<int>(std::min<int64_t>((kSlots / 2 + each - 1) / each, batch));
+    }
   }
   p.most = p.shared_splits + p.own_most;
-  if (p.most > 1) p.partials = T * n_q * p.shared_splits + p.slot_rows * (apart ? p.own_blocks : std::min<int64_t>(p.own_blocks, kSlots));
+  if (p.most > 1)
+    p.partials = T * n_q * p.shared_splits +
+                 p.slot_rows * (apart ? p.own_blocks : std::min<int64_t>(p.own_blocks, p.refill ? 2 * kSlots : kSlots));
   return p;
 }
 
@@ -1011,7 +1060,8 @@ int attn_args(int64_t T, int n_q, int n_kv, int hd, int batch, int L, int shared
   if (T < 0 || T > INT32_MAX || n_q <= 0 || n_kv <= 0 || batch <= 0 || L <= 0 || shared_len < 0 || shared_len > L)
     return Q4_ERR_SHAPE;
   if (L > kMaxKeys) return Q4_ERR_RANGE;
-  if (n_q % n_kv || T * n_q > INT32_MAX) return Q4_ERR_SHAPE;
+  // row numbers of the last tile, and offsets in a token's heads, stay below 2^31
+  if (n_q % n_kv || T * n_q > INT32_MAX - 128 || n_q > INT32_MAX / 2048) return Q4_ERR_SHAPE;
   if (hd != 64 && hd != 128) return Q4_ERR_UNSUPPORTED;
   if (n_q / n_kv > 64) return Q4_ERR_UNSUPPORTED;
   return Q4_OK;
@@ -1079,11 +1129,12 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     a.ml = static_cast<float*>(workspace);
     a.o = a.ml + ml_floats(p.partials);
     a.own = reinterpret_cast<int2*>(a.o + p.partials * hd);
+    a.own_rows = static_cast<int>(p.partials - T * n_q * p.shared_splits);
   }
   a.shared_pages = shared_pages;
   a.T = static_cast<int>(T), a.n_q = n_q, a.n_kv = kv->n_kv, a.g = g, a.L = L, a.shared_len = shared_len;
   a.shared_blocks = static_cast<int>(p.shared_blocks), a.shared_splits = p.shared_splits, a.shared_tile = p.shared_tile;
-  a.own_from = p.own_from, a.slot_rows = p.slot_rows, a.longest_first = p.longest_first;
+  a.own_from = p.own_from, a.slot_rows = p.slot_rows, a.longest_first = p.longest_first, a.refill = p.refill, a.turn_from = p.turn_from;
   // a negative scale turns q around and a zero one clears it, so that the exponents' factor is positive
   a.sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
   a.cs = scale == 0.0f ? 1.0f : std::fabs(scale) * 1.44269504088896340736f;

@@ -292,8 +292,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   }
 }
 
-// Tokens per workgroup and parts per token group: about kU units a thread while that leaves 1024 workgroups (eight
-// rounds of the compute units' four), one token and one unit a thread in a few workgroups.
+// Tokens per workgroup and parts per token group: about kU units a thread while that leaves 1024 workgroups (four for
+// each compute unit), else a token, whose units are split until there are 512.
 struct Split {
   int tpb, part, parts;
 };

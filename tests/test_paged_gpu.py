@@ -435,6 +435,21 @@ def test_paged_attn_more_tiles_than_places(dev, dt, ragged, n, rows, lens, share
         b.check(b.q(n_kv), 0.125, workspace=ws if ws.numel() else None)
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("n,rows,n_kv,hd", [(3, 1, 8, 64), (9, 1, 16, 64), (24, 1, 8, 128), (17, 1, 16, 64), (5, 40, 2, 64),
+                                            (33, 3, 8, 64), (64, 2, 1, 64), (65, 2, 2, 64)])
+def test_paged_attn_unequal_lengths(dev, dt, ragged, n, rows, n_kv, hd):
+    """Sequences of unequal lengths, some empty, in every order of work: few and many of them, tiles that fill the places and
+    tiles that have to be split over them twice."""
+    r = [(0 if i % 11 == 4 else 1 + i % rows) if ragged else rows for i in range(n)]
+    lens = [max(r[i], (37 * i * i + 300 * i) % (1900 if n < 10 else 700)) for i in range(n)]
+    b = Batch(dev, dt, hd, n_kv, 16, lens, r, 0, ragged, seed=n)
+    L = b.page_table.shape[1] * 16
+    ws = torch.full((max(16, ops.paged_attn_workspace_bytes(b.tokens, n_kv, n_kv, hd, n, L, 0)),), 255, dtype=torch.uint8, device=dev)
+    b.check(b.q(n_kv), 0.125, workspace=ws)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 0.01, 2.0])
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 def test_paged_attn_scales(dev, dt, scale):
