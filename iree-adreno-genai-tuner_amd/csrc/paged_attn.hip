@@ -158,43 +158,49 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split,
     item = whole + i;
     if (item >= items) return false;
   }
-  const int tile = a.by_kv.div(item);
+  int tile = a.by_kv.div(item);
   w->h = item - tile * a.n_kv;
-  // Longest first (a batch of 64 at most): those that wait for a place are short. Where none waits and each compute unit gets a
-  // second one, the second ones go shortest first, so that the longest and the shortest share a unit.
-  const int len = lane < a.b.batch && a.longest_first ? a.b.lens[lane] : INT32_MIN;
-  if (!a.b.cu) {
-    int s = a.by_tiles.div(tile);
-    w->tile = tile - s * a.by_tiles.d;
-    if (a.longest_first) {  // the s-th longest
-      if (s >= a.turn_from) s = a.b.batch - 1 - (s - a.turn_from);
-      int rank = 0;
-      for (int l = 0; l < a.b.batch; ++l) {
-        const int o = __builtin_amdgcn_readlane(len, l);
-        rank += o > len || (o == len && l < lane);
+  if (a.longest_first) {
+    // Longest first (a batch of 64 at most): those that wait for a place are short. Where none waits and each compute unit gets
+    // a second one, the second ones go shortest first, so that the longest and the shortest share a unit.
+    int seconds = a.turn_from;
+    if (a.b.cu) {
+      const int per = a.n_kv * w->ranges;
+      seconds = a.shared_blocks == 0 && whole == 0 && items * w->ranges <= kSlots ? (kSlots / 2 + per - 1) / per : INT32_MAX;
+    }
+    if (tile >= seconds) tile = a.by_kv.div(items) - 1 - (tile - seconds);
+    // The sequence that holds this tile of the order, bit by bit of the lengths (in 64 classes: the order need not be exact;
+    // counting for each sequence the longer ones took 2 us of 64 sequences beside the shared keys' work).
+    const int len = lane < a.b.batch ? a.b.lens[lane] : 0, most = a.L - a.own_from;
+    const int n = a.b.cu ? count(0) : lane < a.b.batch ? static_cast<int>(a.by_tiles.d) : 0;
+    const int bits = 32 - __builtin_clz(most), key = min(max(len - a.own_from, 0), most) >> max(bits - 6, 0);
+    auto tiles_in = [&](uint64_t m) -> int {  // bit by bit of their numbers
+      if (!a.b.cu) return __popcll(m) * static_cast<int>(a.by_tiles.d);
+      int sum = 0;
+      for (int i = 0;; ++i) {
+        sum += __popcll(__ballot(n >> i & 1) & m) << i;
+        if (!__ballot(n >> (i + 1))) return sum;
       }
-      s = __builtin_ctzll(__ballot(lane < a.b.batch && rank == s));
+    };
+    uint64_t m = __ballot(n > 0);
+    for (int i = min(bits, 6) - 1; i >= 0; --i) {
+      const uint64_t ones = __ballot(key >> i & 1) & m;
+      const int t = tiles_in(ones);
+      if (tile < t) m = ones;
+      else tile -= t, m &= ~ones;
     }
-    w->seq = s;
-    return true;
+    for (; m; m &= m - 1) {  // equally long
+      w->seq = __builtin_ctzll(m);
+      const int t = __builtin_amdgcn_readlane(n, w->seq);
+      w->tile = tile;
+      if (tile < t) return true;
+      tile -= t;
+    }
+    return false;
   }
-  if (a.longest_first) {  // lane: a sequence, its tiles from `before` on
-    const int n = count(0);
-    int before = 0;
-    for (int l = 0; l < a.b.batch; ++l) {
-      const int o = __builtin_amdgcn_readlane(len, l), t = __builtin_amdgcn_readlane(n, l);
-      before += o > len || (o == len && l < lane) ? t : 0;
-    }
-    if (a.shared_blocks == 0 && whole == 0 && items * w->ranges <= kSlots) {
-      const bool second = before * a.n_kv * w->ranges >= kSlots / 2;
-      int firsts = 0;
-      for (uint64_t m = __ballot(!second && n > 0); m; m &= m - 1) firsts += __builtin_amdgcn_readlane(n, __builtin_ctzll(m));
-      if (second) before = firsts + a.by_kv.div(items) - before - n;
-    }
-    const uint64_t here = __ballot(before <= tile && tile < before + n);
-    if (!here) return false;
-    w->seq = __builtin_ctzll(here);
-    w->tile = tile - __builtin_amdgcn_readlane(before, w->seq);
+  if (!a.b.cu) {
+    w->seq = a.by_tiles.div(tile);
+    w->tile = tile - w->seq * a.by_tiles.d;
     return true;
   }
   int base = 0;
@@ -990,7 +996,7 @@ struct Plan {
   int shared_tile, shared_splits, own_from, slot_rows;
   int places, own_whole, own_items, own_ranges, own_most, own_tiles;  // (without cu_q) tiles of a sequence
   int most;                                                    // ranges of a row at most
-  int turn_from;  // the second ones: sequences from here on
+  int turn_from;  // the second ones: tiles from here on
   bool longest_first, refill;
 };
 
@@ -1037,11 +1043,8 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, 
     // shortest first: 36.0 / 63.2 / 105 and 32.9 / 55.7 / 90 us. Up to three tokens each, 8 KV heads of 128, in the batch's order
     // and so: 38.6 / 64.5 / 109 and 34.8 / 58.0 / 93.
     p.longest_first = batch > 1 && batch <= 64 && keys > 4 * kTurn;
-    p.turn_from = batch;
-    if (!apart && !ragged && p.own_blocks <= kSlots) {
-      const int64_t each = p.own_blocks / batch;
-      p.turn_from = static_cast<int>(std::min<int64_t>((kSlots / 2 + each - 1) / each, batch));
-    }
+    p.turn_from = INT32_MAX;
+    if (!apart && !ragged && p.own_blocks <= kSlots) p.turn_from = (kSlots / 2 + n_kv * p.own_ranges - 1) / (n_kv * p.own_ranges);
   }
   p.most = p.shared_splits + p.own_most;
   if (p.most > 1)
