@@ -73,15 +73,12 @@ struct AttnArgs {
   FastDiv by_g, by_kv, by_shared, by_ranges, by_tiles;
 };
 
-// Rows (token, head of the group) of a workgroup where there are `rows` in all. Up to 32 rows are not enough to share the
+// Rows (token, head of the group) of a workgroup where there are `rows` in all. Up to 16 rows are not enough to share the
 // keys among waves: each wave streams blocks of its own (paged_stream). Past them the waves share stages of keys
-// in LDS (paged_shared), 32 rows a wave: two waves for the rows and two for the keys, or four for the rows. With two
-// terms of q and P (`split`) 32 streamed rows do not fit the registers.
-__host__ __device__ __forceinline__ int tile_rows(int64_t rows, bool split) {
-  if (rows <= 16) return 16;
-  if (rows <= 32 && !split) return 32;
-  return rows <= 64 ? 64 : 128;
-}
+// in LDS (paged_shared), 32 rows a wave: two waves for the rows and two for the keys, or four for the rows. 8 sequences of
+// 1000 to 6000 keys, 32/8 heads of 128, f16 (fp32): 4 rows in tiles of 16 and 64 31.9 and 34.8 us (32.3 and 37.2), 24
+// rows in tiles of 64 and 128 36.9 and 37.9 (39.4 and 44.3), 160 rows in tiles of 64 and 128 73 and 54 (81 and 75).
+__host__ __device__ __forceinline__ int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : 128; }
 
 // The sequence of token t, another in each lane (batch or more: none). Every lane of the wave takes part.
 __device__ __forceinline__ int sequence_of_lane(const PagedBatch& b, int t) {
@@ -102,8 +99,8 @@ __device__ __forceinline__ int2 tokens_of(const PagedBatch& b, int seq, int T) {
   return make_int2(c0, min(max(b.cu[seq + 1], c0), T) - c0);
 }
 
-__host__ __device__ __forceinline__ int tiles_of(int64_t rows, bool split) {
-  const int h = tile_rows(rows, split);
+__host__ __device__ __forceinline__ int tiles_of(int64_t rows) {
+  const int h = tile_rows(rows);
   return static_cast<int>((rows + h - 1) / h);
 }
 
@@ -112,10 +109,11 @@ constexpr int kSlots = 512;    // own ranges at once: two workgroups on every co
 constexpr int kMaxSplits = 64;  // ranges of a tile's keys
 
 // Ranges of each of `items` that share `places`: as many as fit at once, or, where those leave more than an eighth of the
-// places free, as many as fill them twice (the last ones start as the first end; `refill`: not with tiles of the shared
-// form, whose ranges cost more to start: 10 prompts of 100 tokens 72 -> 76 us). One token each of 12 / 20 / 24 sequences of
-// 1000 to 6000 keys, 16 heads of 64: 49.7 / 79.9 / 86.3 -> 43.2 / 64.6 / 87.2 us; 8 KV heads of 128, 24 / 40 sequences:
-// 82 / 138 -> 74 / 115. Where they do fit (8 sequences of 16 heads), the second filling costs: 33.5 -> 34.7 us.
+// places free, as many as fill them twice (the last ones start as the first end; `refill`: of many keys and few rows). One
+// token each of 12 / 20 / 24 sequences of 1000 to 6000 keys, 16 heads of 64: 49.7 / 79.9 / 86.3 -> 43.2 / 64.6 / 87.2 us;
+// 8 KV heads of 128, 24 / 40 sequences: 82 / 138 -> 74 / 115. Where they do fit (8 sequences of 16 heads), the second filling
+// costs: 33.5 -> 34.7 us; so it does for few keys (40 sequences of 1000 keys of 8 heads 27.8 -> 29.2, 2000 keys 45.6 -> 43.2)
+// and for more than 32 rows (80 of 2000 keys 59 -> 64).
 __host__ __device__ __forceinline__ int ranges_of(int items, int places, bool refill, int most) {
   int n = places / items;
   if (refill && 8 * n * items < 7 * places) n = 2 * places / items;
@@ -131,11 +129,11 @@ struct Own {
 };
 
 // Item and range of own workgroup `idx` (wave-uniform); false: none.
-__device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, bool split, Own* w) {
+__device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, Own* w) {
   const int lane = threadIdx.x & 63;
   auto count = [&](int i) {  // lane: tiles of sequence i + lane
     const int s = min(i + lane, a.b.batch - 1);
-    return i + lane < a.b.batch ? tiles_of(static_cast<int64_t>(tokens_of(a.b, s, a.T).y) * a.g, split) : 0;
+    return i + lane < a.b.batch ? tiles_of(static_cast<int64_t>(tokens_of(a.b, s, a.T).y) * a.g) : 0;
   };
   int whole = a.own_whole, items = a.own_items;
   FastDiv by_ranges = a.by_ranges;
@@ -388,7 +386,7 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Item& it, const
   }
 }
 
-// Streaming form: 16 RT rows of one KV head, 32-key blocks dealt to the four waves, which keep (m, l, o) of their own and
+// Streaming form: 16 rows of one KV head, 32-key blocks dealt to the four waves, which keep (m, l, o) of their own and
 // join them at the end. What bounds it is the latency and bandwidth of the key loads.
 //
 // Per block and wave: S^T = K Q^T (16x16x32 MFMA; K straight from memory to the A operand: lane r16 + 16 quad holds key
@@ -396,7 +394,7 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Item& it, const
 // V^T P^T. The S^T accumulators are the P^T operand as they stand: k slots 8 quad + j carry keys 4 quad + j and 16 +
 // 4 quad + j - 4, and V^T comes from a row-major copy of the block in LDS in the same order by transposing reads.
 // The loads of the next block are issued when this one's registers are free, and cross its softmax and PV.
-template <int QT, int CT, int HD, int RT>
+template <int QT, int CT, int HD>
 __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, int entry, unsigned char* buf0,
                                              unsigned char* buf1, float2 (*wml)[64]) {
   typedef vec8<CT> C8;
@@ -406,7 +404,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   constexpr int kCpr = HD / 8;               // 16-byte chunks per row
   constexpr int kVld = kKeys * kCpr / 64;    // V loads per lane
   constexpr int kRpi = 64 / kCpr;            // rows per load instruction
-  constexpr int kBuf = 16 * RT * HD * 4;     // LDS of a wave (two waves a buffer): a V block, then its rows of o
+  constexpr int kBuf = 16 * HD * 4;          // LDS of a wave (two waves a buffer): a V block, then its rows of o
   static_assert(kBuf >= kKeys * kRowB && 2 * kBuf <= 2 * kStage * kRowB, "LDS of a wave");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -448,48 +446,37 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
   }
 
   // The rows, while the first keys are on their way.
-  Row w[RT];
-  C8 qv[RT][KS], ql[RT][kSplit ? KS : 1];
-  int least = INT32_MAX;  // the keys that every row sees
+  const Row w = row_of(a, it, it.row0 + r16);
+  C8 qv[KS], ql[kSplit ? KS : 1];
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    w[x] = row_of(a, it, it.row0 + 16 * x + r16);
-    if (w[x].ok) least = min(least, w[x].lim);
-#pragma unroll
-    for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w[x], 32 * t + 8 * quad, &qv[x][t], &ql[x][kSplit ? t : 0]);
-  }
+  for (int t = 0; t < KS; ++t) load_q<QT, CT>(a, w, 32 * t + 8 * quad, &qv[t], &ql[kSplit ? t : 0]);
+  int least = w.ok ? w.lim : INT32_MAX;  // the keys that every row sees
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) least = min(least, __shfl_xor(least, m, 64));
   least = __builtin_amdgcn_readfirstlane(least);
 
-  f32x4 o[RT][OT];
-  float m[RT], l[RT];  // m in log2 units; l: over this lane's keys
+  f32x4 o[OT];
+  float m = -INFINITY, l = 0.0f;  // m in log2 units; l: over this lane's keys
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    m[x] = -INFINITY, l[x] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < OT; ++d) o[x][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int d = 0; d < OT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   const float neg1 = minus_one();
 
   for (; kb < k1; kb += it.step) {
     // S^T: keys 16 u + 4 quad + i, row r16
-    f32x4 s[RT][2];
+    f32x4 s[2];
 #pragma unroll
-    for (int x = 0; x < RT; ++x)
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 lo = s[u];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[x][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        f32x4 lo = s[x][u];
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-          s[x][u] = mfma16(__builtin_bit_cast(C8, kr[u][t]), qv[x][t], s[x][u]);
-          if constexpr (kSplit) lo = mfma16(__builtin_bit_cast(C8, kr[u][t]), ql[x][t], lo);
-        }
-        if constexpr (kSplit)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[x][u][i] += lo[i];
+      for (int t = 0; t < KS; ++t) {
+        s[u] = mfma16(__builtin_bit_cast(C8, kr[u][t]), qv[t], s[u]);
+        if constexpr (kSplit) lo = mfma16(__builtin_bit_cast(C8, kr[u][t]), ql[t], lo);
       }
+      if constexpr (kSplit)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][i] += lo[i];
+    }
     const uint32_t held = static_cast<uint32_t>(__ballot(slot >= 0));
 #pragma unroll
     for (int i = 0; i < kVld; ++i) {
@@ -501,38 +488,35 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     slot = slot_of(entry, kb + it.step);
     if (kb + it.step < k1) load(slot);
     entry = page_entry(kb + 2 * it.step);
-    C8 ph[RT], pl[RT];
+    C8 ph, pl;
+    if (held != 0xffffffffu || kb + kKeys > least) {
 #pragma unroll
-    for (int x = 0; x < RT; ++x) {
-      if (held != 0xffffffffu || kb + kKeys > least) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = 16 * u + 4 * quad + i;
-            if (kb + k >= w[x].lim || !((held >> k) & 1)) s[x][u][i] = -INFINITY;
-          }
-      }
-      float mb = max3(max3(s[x][0][0], s[x][0][1], s[x][0][2]), max3(s[x][0][3], s[x][1][0], s[x][1][1]),
-                      max3(s[x][1][2], s[x][1][3], s[x][1][3]));
-      mb = swap_combine32<true>(swap_combine16<true>(mb)) * a.cs;
-      // the sums are rescaled only where a maximum has grown by more than 2^8: weights stay below that
-      if (__any(mb > m[x] + 8.0f)) {
-        const float m_new = fmaxf(m[x], mb);
-        const float alpha = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - m_new);
-        m[x] = m_new;
-        l[x] *= alpha;
-#pragma unroll
-        for (int d = 0; d < OT; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[x][d][i] *= alpha;
-      }
-      const float mu = m[x] == -INFINITY ? 0.0f : m[x];
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[x][i >> 2][i & 3], a.cs, -mu));
-      weights8<QT, CT>(p, neg1, &ph[x], &pl[x], &l[x]);
+        for (int i = 0; i < 4; ++i) {
+          const int k = 16 * u + 4 * quad + i;
+          if (kb + k >= w.lim || !((held >> k) & 1)) s[u][i] = -INFINITY;
+        }
     }
+    float mb = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]),
+                    max3(s[1][2], s[1][3], s[1][3]));
+    mb = swap_combine32<true>(swap_combine16<true>(mb)) * a.cs;
+    // the sums are rescaled only where a maximum has grown by more than 2^8: weights stay below that
+    if (__any(mb > m + 8.0f)) {
+      const float m_new = fmaxf(m, mb);
+      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], a.cs, -mu));
+    weights8<QT, CT>(p, neg1, &ph, &pl, &l);
 #pragma unroll
     for (int d = 0; d < OT; ++d) {
       short4v v[2];
@@ -542,61 +526,50 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
         v[u] = read_tr4(vb + r * kRowB + ((c ^ vswz<HD>(r)) << 4) + (r16 & 1) * 8);
       }
       const C8 va = __builtin_bit_cast(C8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        o[x][d] = mfma16(va, ph[x], o[x][d]);
-        if constexpr (kSplit) o[x][d] = mfma16(va, pl[x], o[x][d]);
-      }
+      o[d] = mfma16(va, ph, o[d]);
+      if constexpr (kSplit) o[d] = mfma16(va, pl, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 
   // Join the four waves: (m, l) of each, then the weighted o.
-#pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    l[x] = swap_combine32<false>(swap_combine16<false>(l[x]));
-    if (l[x] != l[x] && m[x] == -INFINITY) m[x] = 0.0f;  // every score was NaN: not a range without keys
-    if (quad == 0) wml[wave][16 * x + r16] = make_float2(m[x], l[x]);
-  }
+  l = swap_combine32<false>(swap_combine16<false>(l));
+  if (l != l && m == -INFINITY) m = 0.0f;  // every score was NaN: not a range without keys
+  if (quad == 0) wml[wave][r16] = make_float2(m, l);
   __syncthreads();
   float* jb = reinterpret_cast<float*>(vb);  // rows of HD floats, their 16-byte chunks swizzled by the row
+  float M = wml[0][r16].x;
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    float M = wml[0][16 * x + r16].x;
+  for (int v = 1; v < kWaves; ++v) M = fmaxf(M, wml[v][r16].x);
+  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  if (w.ok) {
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) M = fmaxf(M, wml[v][16 * x + r16].x);
-    const float f = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
-    if (w[x].ok) {
-#pragma unroll
-      for (int d = 0; d < OT; ++d)
-        *reinterpret_cast<f32x4*>(jb + (16 * x + r16) * HD + 4 * ((4 * d + quad) ^ r16)) =
-            f32x4{f * o[x][d][0], f * o[x][d][1], f * o[x][d][2], f * o[x][d][3]};
-    }
+    for (int d = 0; d < OT; ++d)
+      *reinterpret_cast<f32x4*>(jb + r16 * HD + 4 * ((4 * d + quad) ^ r16)) =
+          f32x4{f * o[d][0], f * o[d][1], f * o[d][2], f * o[d][3]};
   }
   __syncthreads();
-  // thread: row r, dims 4 c ..; a row's place is that of lane r % 16 (all lanes take part in the shuffles: kC4 is 16 or 32)
+  // thread: row r, dims 4 c ..; a row's place is that of lane r (all lanes take part in the shuffles: kC4 is 16 or 32)
   constexpr int kC4 = HD / 4;
+  for (int e = threadIdx.x; e < 16 * kC4; e += kThreads) {
+    const int r = e / kC4, c = e % kC4;
+    Row y;
+    y.token = __shfl(w.token, r, 64), y.head = __shfl(w.head, r, 64), y.in_tile = r;
+    if (!__shfl(static_cast<int>(w.ok), r, 64)) continue;
+    float mm = wml[0][r].x;
 #pragma unroll
-  for (int x = 0; x < RT; ++x)
-    for (int e = threadIdx.x; e < 16 * kC4; e += kThreads) {
-      const int r = e / kC4, c = e % kC4;
-      Row y;
-      y.token = __shfl(w[x].token, r, 64), y.head = __shfl(w[x].head, r, 64), y.in_tile = 16 * x + r;
-      if (!__shfl(static_cast<int>(w[x].ok), r, 64)) continue;
-      float mm = wml[0][16 * x + r].x;
+    for (int v = 1; v < kWaves; ++v) mm = fmaxf(mm, wml[v][r].x);
+    float den = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int v = 1; v < kWaves; ++v) mm = fmaxf(mm, wml[v][16 * x + r].x);
-      float den = 0.0f;
-      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        const float2 z = wml[i][16 * x + r];
-        den += z.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z.x - mm) * z.y;
-        v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf_of(i)) + (16 * x + r) * HD + 4 * (c ^ r));
-      }
-      const float y4[4] = {v[0], v[1], v[2], v[3]};
-      store_o<QT, HD, 4>(a, it, y, 4 * c, y4, mm, den);
+    for (int i = 0; i < kWaves; ++i) {
+      const float2 z = wml[i][r];
+      den += z.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(z.x - mm) * z.y;
+      v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(buf_of(i)) + r * HD + 4 * (c ^ r));
     }
+    const float y4[4] = {v[0], v[1], v[2], v[3]};
+    store_o<QT, HD, 4>(a, it, y, 4 * c, y4, mm, den);
+  }
 }
 
 // 16 bytes per lane from memory straight into LDS (lane i's at dst + 16 i).
@@ -862,7 +835,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     it.n_rows = a.T * a.g;
   } else {
     Own w;
-    if (!own_item(a, idx, QT == Q4_F32, &w)) return;
+    if (!own_item(a, idx, &w)) return;
     it.h = __builtin_amdgcn_readfirstlane(w.h);
     it.seq = __builtin_amdgcn_readfirstlane(w.seq);
     it.ranges = w.ranges, it.slot0 = w.slot0;
@@ -871,10 +844,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     const int2 tk = tokens_of(a.b, it.seq, a.T);
     it.tok0 = tk.x;
     it.n_rows = tk.y * a.g;
-    height = tile_rows(it.n_rows, QT == Q4_F32);
+    height = tile_rows(it.n_rows);
     it.table += it.seq * a.b.stride;
   }
-  const bool stream = height <= 32;
+  const bool stream = height == 16;
   const int turn = stream ? kTurn : kStage;
   it.row0 = tile * height;
   it.k0 = (it.shared ? 0 : a.own_from) + split * turn;
@@ -894,9 +867,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
     if (split >= it.ranges) return;
   }
   it.step = it.ranges * turn;
-  if (height == 16) return paged_stream<QT, CT, HD, 1>(a, it, entry, buf0, buf1, wml);
-  if constexpr (QT != Q4_F32)
-    if (height == 32) return paged_stream<QT, CT, HD, 2>(a, it, entry, buf0, buf1, wml);
+  if (stream) return paged_stream<QT, CT, HD>(a, it, entry, buf0, buf1, wml);
   if (height == 64) paged_shared<QT, CT, HD, 2>(a, it, entry, buf0, buf1, wml);
   else paged_shared<QT, CT, HD, 4>(a, it, entry, buf0, buf1, wml);
 }
@@ -1000,7 +971,7 @@ struct Plan {
   bool longest_first, refill;
 };
 
-Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, int L, int shared_len) {
+Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int shared_len) {
   Plan p{};
   const int g = n_q / n_kv;
   const int64_t rows = T * g;
@@ -1014,30 +985,37 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, bool split, 
   if (apart) {
     // One workgroup for every compute unit: the other place of each is left to own ranges, and what ranges write and the join
     // reads stays small (of 48 x 5 tokens x 32 heads and 4096 shared keys, 17 MB; with two 73 us, with one 62).
-    p.shared_tile = tile_rows(rows, split);
-    const int64_t items = n_kv * static_cast<int64_t>(tiles_of(rows, split));
+    p.shared_tile = tile_rows(rows);
+    const int64_t items = n_kv * static_cast<int64_t>(tiles_of(rows));
     p.shared_splits = static_cast<int>(std::max<int64_t>(
         1, std::min<int64_t>({kSlots / 2 / items, (shared_len + kTurn - 1) / kTurn, kMaxSplits})));
     p.shared_blocks = items * p.shared_splits;
   }
   p.places = kSlots - static_cast<int>(std::min<int64_t>(p.shared_blocks, kSlots / 2));  // what shared ranges leave
   if (const int64_t keys = L - p.own_from; keys > 0) {
-    p.refill = rows / batch <= 32;  // (of sequences of different lengths: the mean)
+    // (with cu_q, which only the device reads, these go by the mean of the rows and by one tile for each sequence)
+    p.refill = rows / batch <= 32 && keys >= 2048;
+    p.own_tiles = ragged ? 1 : tiles_of(rows / batch);
+    const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv;
     const int slots = p.refill ? 2 * kSlots : kSlots;
-    p.own_most = static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
+    // Short keys are one range, which needs no join: up to two blocks a wave always, up to four where there are items for a
+    // quarter of the units. One token each of 1 / 4 / 12 / 32 sequences, 8 KV heads of 128, one range and as many as fit:
+    // 250 keys 7.8 / 7.9 / 8.9 / 10.5 and 8.8 / 8.8 / 10.6 / 13.6 us, 400 keys 9.9 / 10.0 / 11.4 / 14.1 and 8.9 / 10.0 /
+    // 12.5 / 16.9.
+    const bool one = !apart && keys <= (items >= kSlots / 8 ? 4 : 2) * kTurn;
+    p.own_most = one ? 1 : static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
     if (ragged) {
       // the number of tiles, and so of ranges, is known on the device alone; at most one tile that is not full a sequence, and
       // a full one has 128 rows
       p.own_blocks = (rows / 128 + batch) * n_kv + slots;
-      p.slot_rows = tile_rows(rows, split);
+      p.slot_rows = tile_rows(rows);
     } else {
-      p.own_tiles = tiles_of(rows / batch, split);
-      const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv, rest = items % kSlots;
+      const int64_t rest = items % kSlots;
       p.own_ranges = rest ? ranges_of(static_cast<int>(rest), p.places, p.refill, p.own_most) : 1;
       p.own_items = static_cast<int>(items), p.own_whole = static_cast<int>(items - rest);
       p.own_blocks = items - rest + rest * p.own_ranges;
       p.own_most = p.own_ranges;
-      p.slot_rows = tile_rows(rows / batch, split);
+      p.slot_rows = tile_rows(rows / batch);
     }
     // One token each of 8 / 16 / 28 sequences of 1000 to 6000 keys, 16 heads of 64, the second ones longest first too and
     // shortest first: 36.0 / 63.2 / 105 and 32.9 / 55.7 / 90 us. Up to three tokens each, 8 KV heads of 128, in the batch's order
@@ -1094,10 +1072,9 @@ extern "C" int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head
   if (!bytes) return Q4_ERR_NULL;
   if (int st = attn_args(T, n_q, n_kv, head_dim, batch, L, shared_len)) return st;
   size_t most = 0;
-  for (const int form : {0, 1, 2, 3}) {  // cu_q or not, fp32 or not
-    const bool ragged = form & 1, split = form & 2;
+  for (const bool ragged : {false, true}) {  // with cu_q or not
     if (!ragged && T % batch) continue;
-    most = std::max(most, workspace_of(plan_for(T, n_q, n_kv, batch, ragged, split, L, shared_len), T * n_q, head_dim));
+    most = std::max(most, workspace_of(plan_for(T, n_q, n_kv, batch, ragged, L, shared_len), T * n_q, head_dim));
   }
   *bytes = most;
   return Q4_OK;
@@ -1119,7 +1096,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     return Q4_ERR_ALIGN;
   if (T == 0) return Q4_OK;
   const int g = n_q / kv->n_kv;
-  const Plan p = plan_for(T, n_q, kv->n_kv, kv->batch, kv->cu_q != nullptr, dtype == Q4_F32, L, shared_len);
+  const Plan p = plan_for(T, n_q, kv->n_kv, kv->batch, kv->cu_q != nullptr, L, shared_len);
   if (p.partials) {
     if (!workspace || workspace_bytes < workspace_of(p, T * n_q, hd)) return Q4_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return Q4_ERR_ALIGN;
