@@ -315,7 +315,7 @@ typedef struct q4_rope {
  * gradient of x from that of y). x, y: T x heads x head_dim of dtype (F32, F16, BF16), rows and heads
  * *_row and *_head elements apart (>= 0), the dims of a head next to each other. y may be x itself (same
  * strides); other overlaps are not allowed. Arithmetic in fp32, one rounding. head_dim even and <= 1024,
- * rot_dim even and <= head_dim, T * heads < 2^31. T == 0 does nothing. */
+ * rot_dim even and <= head_dim, T * heads < 2^31, heads * head_dim < 2^27. T == 0 does nothing. */
 int rope_rotate(const void* x, int64_t x_row, int64_t x_head, void* y, int64_t y_row, int64_t y_head, int dtype,
                 int64_t T, int heads, int head_dim, const int32_t* positions, const q4_rope* rope, int inverse,
                 void* stream);
@@ -364,9 +364,9 @@ int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int b
  * Rows of the cache that hold no key of a sequence may hold anything; the values of keys 0 .. seq_lens - 1 and of the
  * shared keys are finite, also those that a token does not see (a NaN there can reach tokens before it). q_row and
  * q_head: elements between rows and heads, q and the strides multiples of 16 bytes, caches and out
- * 16-byte aligned; out overlaps neither q nor the caches. Requires n_q % n_kv == 0, n_q / n_kv <= 64, head_dim 64 or
- * 128, 0 < L <= 2^30, 0 <= shared_len <= L, a finite scale, shared_len <= num_pages * page_size. Keys at or past L are
- * not read. */
+ * 16-byte aligned; out overlaps neither q nor the caches; calls that may run at once need workspaces of their own. Requires
+ * n_q % n_kv == 0, n_q / n_kv <= 64, n_q < 2^20, T * n_q < 2^31 - 128, head_dim 64 or 128, 0 < L <= 2^30,
+ * 0 <= shared_len <= L, a finite scale, shared_len <= num_pages * page_size. Keys at or past L are not read. */
 int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, int64_t q_head, void* out, int dtype, int64_t T,
                int n_q, int L, const int32_t* shared_pages, int shared_len, float scale, void* workspace,
                size_t workspace_bytes, void* stream);
@@ -380,7 +380,7 @@ int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, int64_t q_he
  * positive w, and -1 when w is zero everywhere. draft NULL: the drafts are certain (probability 1 at the
  * token, 0 elsewhere). Negative and NaN weights count as zero. out_tokens [B, K + 1]: the accepted tokens, the
  * next one, then -1; n_accepted [B]. Products and sums are fp64, in a fixed order. A drafted token outside
- * [0, V) is refused. Strides in elements; rows of V next to each other. Requires B > 0, K >= 0, 0 < V < 2^31. */
+ * [0, V) is refused. Strides in elements; rows of V next to each other. Requires B > 0, K >= 0, 0 < V < 2^31 - 1024. */
 int spec_verify_workspace_bytes(int B, int K, int64_t V, size_t* bytes);
 int spec_verify(const int32_t* tokens, int64_t tok_row, const float* draft, int64_t draft_batch, int64_t draft_row,
                 const float* target, int64_t target_batch, int64_t target_row, const float* uniforms, int64_t uni_row,
