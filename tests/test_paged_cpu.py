@@ -96,6 +96,21 @@ def test_paged_attn_refuses_a_workspace(bad, code, shared):
     assert attend(**big, nbytes=64) == ERR["WORKSPACE"]
 
 
+@pytest.mark.parametrize("T,n_q,n_kv,code", [(1, 1 << 20, 1 << 20, "SHAPE"), (1, (1 << 20) - 1, (1 << 20) - 1, None),
+                                             ((1 << 31) - 128, 1, 1, "SHAPE"), ((1 << 31) - 129, 1, 1, None), (1 << 26, 64, 1, "SHAPE")])
+def test_paged_attn_limits_of_rows_and_heads(T, n_q, n_kv, code):
+    b = C.c_size_t(0)
+    assert LIB.raw("paged_attn_workspace_bytes")(T, n_q, n_kv, 128, 1, 256, 0, C.byref(b)) == (ERR[code] if code else 0)
+
+
+def test_paged_attn_short_keys_need_no_workspace():
+    """One range writes the result itself: up to 256 keys, up to 512 where the batch has 64 tiles of rows and heads."""
+    need = LIB.raw("paged_attn_workspace_bytes")
+    for batch, n_kv, L, some in ((1, 8, 256, False), (1, 8, 257, True), (7, 8, 512, True), (8, 8, 512, False), (8, 8, 513, True)):
+        b = C.c_size_t(0)
+        assert need(batch, 4 * n_kv, n_kv, 128, batch, L, 0, C.byref(b)) == 0 and (b.value > 0) == some, (batch, L)
+
+
 def verify(tok=FAKE, draft=FAKE, target=FAKE, u=FAKE, nd=None, B=2, K=3, V=100, out=FAKE, acc=FAKE, ws=FAKE, nbytes=1 << 20,
            strides=(3, 300, 100, 400, 100, 4)):
     s = strides
