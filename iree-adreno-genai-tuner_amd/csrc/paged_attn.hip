@@ -117,7 +117,13 @@ constexpr int kMaxSplits = 64;  // ranges of a tile's keys
 // 8 KV heads of 128, 24 / 40 sequences: 82 / 138 -> 74 / 115. Where they do fit (8 sequences of 16 heads), the second filling
 // costs: 33.5 -> 34.7 us; so it does for few keys (40 sequences of 1000 keys of 8 heads 27.8 -> 29.2, 2000 keys 45.6 -> 43.2)
 // and for more than 32 rows (80 of 2000 keys 59 -> 64).
-__host__ __device__ __forceinline__ int ranges_of(int items, int places, bool refill, int most) {
+//
+// One each where the free places times the keys are few (no shared ranges, which need a join anyway): what splitting saves of the
+// time of an item, the free share of it, has to exceed what ranges cost, about that of 520 keys. 600 keys, 8 KV heads of 128,
+// 24 sequences of 1 / 30 / 100 tokens 19.2 / 35.2 / 65.9 -> 16.0 / 25.5 / 53 us; 2 of them 9.9 / 17.0 / 24.0 as they are, 11.9 /
+// 21.3 / 22.3 in one; 1000 keys, 8 and 24 of 100 tokens 38.4 / 90 -> 34.7 / 78.
+__host__ __device__ __forceinline__ int ranges_of(int items, int places, bool refill, int most, int keys) {
+  if (places == kSlots && keys > 4 * kTurn && static_cast<int64_t>(places - items) * keys <= places * 520) return 1;
   int n = places / items;
   if (refill && 8 * n * items < 7 * places) n = 2 * places / items;
   return n < 1 ? 1 : n < most ? n : most;
@@ -147,7 +153,7 @@ __device__ __forceinline__ bool own_item(const AttnArgs& a, int idx, Own* w) {
     for (int m = 32; m >= 1; m >>= 1) tiles += __shfl_xor(tiles, m, 64);
     items = __builtin_amdgcn_readfirstlane(tiles) * a.n_kv;
     whole = items / kSlots * kSlots;
-    by_ranges.d = ranges_of(max(items - whole, 1), a.places, a.refill, a.own_most);
+    by_ranges.d = ranges_of(max(items - whole, 1), a.places, a.refill, a.own_most, a.L - a.own_from);
   }
   int item = idx;
   w->range = 0, w->ranges = 1, w->slot0 = idx;
@@ -1018,7 +1024,7 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
       p.slot_rows = tile_rows(rows);
     } else {
       const int64_t rest = items % kSlots;
-      p.own_ranges = rest ? ranges_of(static_cast<int>(rest), p.places, p.refill, p.own_most) : 1;
+      p.own_ranges = rest ? ranges_of(static_cast<int>(rest), p.places, p.refill, p.own_most, static_cast<int>(keys)) : 1;
       p.own_items = static_cast<int>(items), p.own_whole = static_cast<int>(items - rest);
       p.own_blocks = items - rest + rest * p.own_ranges;
       p.own_most = p.own_ranges;
