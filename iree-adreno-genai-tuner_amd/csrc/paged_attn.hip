@@ -1038,6 +1038,7 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
     if (!apart && !ragged && p.own_blocks <= kSlots) p.turn_from = (kSlots / 2 + n_kv * p.own_ranges - 1) / (n_kv * p.own_ranges);
   }
   p.most = p.shared_splits + p.own_most;
+  if (apart) p.most = std::max(p.most, 2);  // shared ranges are joined also where a row has one range in all (L == shared_len)
   if (p.most > 1)
     p.partials = T * n_q * p.shared_splits +
                  p.slot_rows * (apart ? p.own_blocks : std::min<int64_t>(p.own_blocks, p.refill ? 2 * kSlots : kSlots));

@@ -111,6 +111,14 @@ def test_paged_attn_short_keys_need_no_workspace():
         assert need(batch, 4 * n_kv, n_kv, 128, batch, L, 0, C.byref(b)) == 0 and (b.value > 0) == some, (batch, L)
 
 
+def test_paged_attn_shared_keys_alone_need_a_workspace():
+    """Where no key is a sequence's own (L == shared_len) and there are tiles enough for one range of the shared keys."""
+    for batch in (2, 40, 640, 2000):
+        b = C.c_size_t(0)
+        assert LIB.raw("paged_attn_workspace_bytes")(batch, 32, 8, 128, batch, 512, 512, C.byref(b)) == 0
+        assert b.value >= batch * 32 * (128 + 2) * 4, batch
+
+
 def verify(tok=FAKE, draft=FAKE, target=FAKE, u=FAKE, nd=None, B=2, K=3, V=100, out=FAKE, acc=FAKE, ws=FAKE, nbytes=1 << 20,
            strides=(3, 300, 100, 400, 100, 4)):
     s = strides

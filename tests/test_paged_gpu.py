@@ -450,6 +450,25 @@ def test_paged_attn_unequal_lengths(dev, dt, ragged, n, rows, n_kv, hd):
     b.check(b.q(n_kv), 0.125, workspace=ws)
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,n_q,n_kv", [(2, 4, 2), (70, 32, 32), (700, 32, 16)])
+def test_paged_attn_shared_keys_alone(dev, dt, n, n_q, n_kv):
+    """No key is a sequence's own: few tiles, whose shared keys are several ranges, and more tiles than compute units, whose
+    shared keys are one."""
+    b = Batch(dev, dt, 64, n_kv, 16, [520 + (i % 2) for i in range(n)], [1] * n, 512, seed=n)
+    q = b.q(n_q)
+    L = 512
+    ws = torch.full((ops.paged_attn_workspace_bytes(n, n_q, n_kv, 64, n, L, 512),), 255, dtype=torch.uint8, device=dev)
+    got = ops.paged_attn(q, b.k, b.v, b.page_table, b.seq_lens, 0.125, shared_pages=b.sp, shared_len=512, L=L, workspace=ws)
+    at = torch.tensor(b.shared_pages, device=dev)
+    k, v = (x[at].flatten(0, 1).double().repeat_interleave(n_q // n_kv, 1) for x in (b.k, b.v))  # [512, n_q, hd]
+    s = torch.einsum("thd,jhd->thj", q.double().cpu(), k.cpu()) * 0.125
+    ref = torch.einsum("thj,jhd->thd", s.softmax(-1), v.cpu()).flatten(1)
+    # the weights' rounding and the result's, each half a step of at most max |v|; scores of 64 products in fp32, off by at
+    # most 66 U sum |q k| scale < 66 U * 200 / 8 = 1e-4 (sum |q k| < 200: 64 normal pairs of mean 0.64), as is e^s
+    assert (got.double().cpu() - ref).abs().max() <= (2 * half_step(dt) + 2e-4) * v.abs().max().item()
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 0.01, 2.0])
 @pytest.mark.parametrize("dt", DTYPES, ids=IDS)
 def test_paged_attn_scales(dev, dt, scale):
