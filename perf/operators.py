@@ -15,8 +15,6 @@ import torch
 
 own = False
 
-PACKAGE = str(pathlib.Path(__file__).resolve().parent.parent / "iree-adreno-genai-tuner_amd")
-
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 CACHE = {"f32": torch.float16, "f16": torch.float16, "bf16": torch.bfloat16}  # activations -> cache
 
@@ -237,8 +235,9 @@ def run(state):
 
 
 def _run_own(s):
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    package = str(pathlib.Path(__file__).resolve().parent.parent / "iree-adreno-genai-tuner_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     from q4llm import ops
     from q4llm.rope import Rope
     c = s["case"]
