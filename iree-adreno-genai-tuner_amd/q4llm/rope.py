@@ -74,8 +74,8 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
       linear            frequencies / factor (position interpolation)
       dynamic           base grown with seq_len past the trained length (NTK-aware scaling)
       yarn              frequencies of long wavelengths interpolated, those of short ones kept, in between a ramp over
-                        the dims from beta_fast to beta_slow turns within the trained length; cos and sin times
-                        attention_factor, or 0.1 ln(factor) + 1 (Peng et al. 2023)
+                        the dims from beta_fast to beta_slow turns within the trained length; cos and sin times attention_factor, or m(mscale) / m(mscale_all_dim) where both are
+                        given, else m(1), with m(x) = 0.1 x ln(factor) + 1 (Peng et al. 2023)
     on the host; `.to(device)` for the operators."""
     p = _rope_params(cfg)
     hd = cfg.get("head_dim") or cfg["hidden_size"] // cfg["num_attention_heads"]
@@ -103,5 +103,7 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
     inv = 1.0 / (base ** exps)
     mscale = p.get("attention_factor")
     if mscale is None:
-        mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        m = lambda x: 0.1 * x * math.log(factor) + 1.0 if factor > 1 else 1.0  # noqa: E731
+        one, all_dim = p.get("mscale"), p.get("mscale_all_dim")
+        mscale = m(one) / m(all_dim) if one and all_dim else m(1.0)
     return Rope(inv / factor * ramp + inv * (1 - ramp), interleaved, float(mscale))
