@@ -74,7 +74,8 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
       linear            frequencies / factor (position interpolation)
       dynamic           base grown with seq_len past the trained length (NTK-aware scaling)
       yarn              frequencies of long wavelengths interpolated, those of short ones kept, in between a ramp over
-                        the dims from beta_fast to beta_slow turns within the trained length; cos and sin times attention_factor, or m(mscale) / m(mscale_all_dim) where both are
+                        the dims from beta_fast to beta_slow turns within the trained length (whole dims unless truncate
+                        is false); cos and sin times attention_factor, or m(mscale) / m(mscale_all_dim) where both are
                         given, else m(1), with m(x) = 0.1 x ln(factor) + 1 (Peng et al. 2023)
     on the host; `.to(device)` for the operators."""
     p = _rope_params(cfg)
@@ -97,8 +98,10 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
     def dim_of(turns):  # the dim whose wavelength makes `turns` turns within the trained length
         return d * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    lo = max(math.floor(dim_of(p.get("beta_fast") or 32)), 0)
-    hi = min(math.ceil(dim_of(p.get("beta_slow") or 1)), d - 1)
+    lo, hi = dim_of(p.get("beta_fast") or 32), dim_of(p.get("beta_slow") or 1)
+    if p.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, d - 1)
     ramp = ((torch.arange(d // 2, dtype=torch.float) - lo) / (hi - lo if hi != lo else 0.001)).clamp(0, 1)
     inv = 1.0 / (base ** exps)
     mscale = p.get("attention_factor")

@@ -29,7 +29,8 @@ def yarn(d, theta, factor, trained, fast=32, slow=1, truncate=True):
     (dict(mscale=1.0, mscale_all_dim=1.0), 1.0),
     (dict(mscale=1.0, mscale_all_dim=0.5), (0.1 * math.log(40) + 1) / (0.05 * math.log(40) + 1)),
     (dict(mscale=0.707), 0.1 * math.log(40) + 1), (dict(mscale_all_dim=0.707), 0.1 * math.log(40) + 1),
-    (dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.1), 1.1), (dict(beta_fast=20, beta_slow=2), 0.1 * math.log(40) + 1)])
+    (dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.1), 1.1), (dict(truncate=False), 0.1 * math.log(40) + 1),
+    (dict(truncate=False, beta_fast=20, beta_slow=2), 0.1 * math.log(40) + 1), (dict(truncate=True), 0.1 * math.log(40) + 1)])
 def test_yarn_keys(keys, mscale, theta):
     got = rope_params({**CFG, "rope_theta": theta, "rope_scaling": {
         "rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 2048, **keys}})
@@ -42,7 +43,7 @@ def test_yarn_keys(keys, mscale, theta):
 
 @pytest.mark.parametrize("scaling", [
     {"rope_type": "yarn", "factor": 40.0, "mscale": 1.0, "mscale_all_dim": 0.5, "original_max_position_embeddings": 2048},
-    {"rope_type": "yarn", "factor": 40.0, "mscale": 0.707}])
+    {"rope_type": "yarn", "factor": 40.0, "mscale": 0.707}, {"rope_type": "yarn", "factor": 32.0, "truncate": False}])
 def test_the_same_as_transformers(scaling):
     pytest.importorskip("transformers")
     from transformers import LlamaConfig
