@@ -72,7 +72,7 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
     """The Rope of a model config: partial heads (partial_rotary_factor) and the scalings for long contexts
       default, llama3   as inv_freq
       linear            frequencies / factor (position interpolation)
-      dynamic           base grown with seq_len past the trained length (NTK-aware scaling)
+      dynamic           base grown with seq_len past max_position_embeddings (NTK-aware scaling)
       yarn              frequencies of long wavelengths interpolated, those of short ones kept, in between a ramp over
                         the dims from beta_fast to beta_slow turns within the trained length (whole dims unless truncate
                         is false); cos and sin times attention_factor, or m(mscale) / m(mscale_all_dim) where both are
@@ -86,14 +86,15 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
         return Rope(inv_freq({**cfg, "head_dim": d}), interleaved)
     base, factor = p["rope_theta"], p["factor"]
     exps = torch.arange(0, d, 2, dtype=torch.int64).to(dtype=torch.float) / d
-    trained = p.get("original_max_position_embeddings") or cfg["max_position_embeddings"]
     if kind == "linear":
         return Rope(1.0 / (base ** exps) / factor, interleaved)
     if kind == "dynamic":
+        trained = cfg["max_position_embeddings"]
         n = max(seq_len or trained, trained)
         return Rope(1.0 / ((base * ((factor * n / trained) - (factor - 1)) ** (d / (d - 2))) ** exps), interleaved)
     if kind != "yarn":
         raise NotImplementedError(f"rope_type {kind!r}")
+    trained = p.get("original_max_position_embeddings") or cfg["max_position_embeddings"]
 
     def dim_of(turns):  # the dim whose wavelength makes `turns` turns within the trained length
         return d * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))

@@ -41,9 +41,22 @@ def test_yarn_keys(keys, mscale, theta):
     assert abs(got.mscale - mscale) <= 1e-12
 
 
+def test_dynamic_grows_from_the_config_length():
+    """max_position_embeddings is the length that the base is kept to, whatever original_max_position_embeddings says."""
+    for n in (100, 3000, 4096, 10000):
+        plain = rope_params({**CFG, "rope_scaling": {"rope_type": "dynamic", "factor": 2.0}}, seq_len=n)
+        given = rope_params({**CFG, "rope_scaling": {"rope_type": "dynamic", "factor": 2.0,
+                                                     "original_max_position_embeddings": 2048}}, seq_len=n)
+        assert torch.equal(plain.inv_freq, given.inv_freq)
+        base = 10000.0 * (2.0 * max(n, 4096) / 4096 - 1) ** (64 / 62)
+        want = base ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+        assert ((given.inv_freq.double() - want).abs() <= 32 * 2.0 ** -24 * want).all()
+
+
 @pytest.mark.parametrize("scaling", [
     {"rope_type": "yarn", "factor": 40.0, "mscale": 1.0, "mscale_all_dim": 0.5, "original_max_position_embeddings": 2048},
-    {"rope_type": "yarn", "factor": 40.0, "mscale": 0.707}, {"rope_type": "yarn", "factor": 32.0, "truncate": False}])
+    {"rope_type": "yarn", "factor": 40.0, "mscale": 0.707}, {"rope_type": "yarn", "factor": 32.0, "truncate": False},
+    {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048}])
 def test_the_same_as_transformers(scaling):
     pytest.importorskip("transformers")
     from transformers import LlamaConfig
