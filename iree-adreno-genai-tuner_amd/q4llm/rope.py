@@ -68,6 +68,12 @@ def rope_tables(cfg: dict, max_ctx: int):
     return emb.cos() * 1.0, emb.sin() * 1.0
 
 
+# The keys of a config's scaling that rope_params goes by (some have no effect on a type and are often there all the same).
+_ROPE_KEYS = {"rope_type", "type", "rope_theta", "factor", "original_max_position_embeddings", "partial_rotary_factor"}
+_SCALING_KEYS = {"default": set(), "linear": set(), "dynamic": set(), "llama3": {"low_freq_factor", "high_freq_factor"},
+                 "yarn": {"beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"}}
+
+
 def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Rope:
     """The Rope of a model config: partial heads (partial_rotary_factor) and the scalings for long contexts
       default, llama3   as inv_freq
@@ -77,11 +83,17 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
                         the dims from beta_fast to beta_slow turns within the trained length (whole dims unless truncate
                         is false); cos and sin times attention_factor, or m(mscale) / m(mscale_all_dim) where both are
                         given, else m(1), with m(x) = 0.1 x ln(factor) + 1 (Peng et al. 2023)
-    on the host; `.to(device)` for the operators."""
+    on the host; `.to(device)` for the operators. NotImplementedError for other types and for scaling keys that are not
+    known here, which might change the frequencies."""
     p = _rope_params(cfg)
     hd = cfg.get("head_dim") or cfg["hidden_size"] // cfg["num_attention_heads"]
     d = int(hd * p.get("partial_rotary_factor", cfg.get("partial_rotary_factor", 1.0)))
     kind = p["rope_type"]
+    if kind not in _SCALING_KEYS:
+        raise NotImplementedError(f"rope_type {kind!r}")
+    unknown = sorted(k for k, x in p.items() if x is not None and k not in _ROPE_KEYS | _SCALING_KEYS[kind])
+    if unknown:
+        raise NotImplementedError(f"rope_type {kind!r} with {', '.join(unknown)}")
     if kind in ("default", "llama3"):
         return Rope(inv_freq({**cfg, "head_dim": d}), interleaved)
     base, factor = p["rope_theta"], p["factor"]
@@ -92,8 +104,6 @@ def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Ro
         trained = cfg["max_position_embeddings"]
         n = max(seq_len or trained, trained)
         return Rope(1.0 / ((base * ((factor * n / trained) - (factor - 1)) ** (d / (d - 2))) ** exps), interleaved)
-    if kind != "yarn":
-        raise NotImplementedError(f"rope_type {kind!r}")
     trained = p.get("original_max_position_embeddings") or cfg["max_position_embeddings"]
 
     def dim_of(turns):  # the dim whose wavelength makes `turns` turns within the trained length

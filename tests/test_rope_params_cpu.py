@@ -54,6 +54,23 @@ def test_dynamic_grows_from_the_config_length():
 
 
 @pytest.mark.parametrize("scaling", [
+    {"rope_type": "yarn", "factor": 4.0, "short_factor": [1.0]}, {"rope_type": "default", "mrope_section": [16, 8, 8]},
+    {"rope_type": "linear", "factor": 2.0, "truncate": False}, {"rope_type": "longrope", "factor": 2.0},
+    {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "mscale": 2.0,
+     "original_max_position_embeddings": 1024}])
+def test_unknown_keys_are_refused(scaling):
+    with pytest.raises(NotImplementedError):
+        rope_params({**CFG, "rope_scaling": scaling})
+
+
+def test_keys_without_a_value_are_none():
+    a = rope_params({**CFG, "rope_scaling": {"rope_type": "yarn", "factor": 4.0}})
+    b = rope_params({**CFG, "rope_scaling": {"type": "yarn", "rope_type": "yarn", "factor": 4.0, "mscale": None, "attention_factor": None,
+                                             "short_factor": None}})
+    assert torch.equal(a.inv_freq, b.inv_freq) and a.mscale == b.mscale
+
+
+@pytest.mark.parametrize("scaling", [
     {"rope_type": "yarn", "factor": 40.0, "mscale": 1.0, "mscale_all_dim": 0.5, "original_max_position_embeddings": 2048},
     {"rope_type": "yarn", "factor": 40.0, "mscale": 0.707}, {"rope_type": "yarn", "factor": 32.0, "truncate": False},
     {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048}])
