@@ -48,6 +48,12 @@ __device__ __forceinline__ f32x16 mfma32(vec8<Q4_BF16> a, vec8<Q4_BF16> b, f32x1
 __device__ __forceinline__ short4v read_tr4(const void* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
 }
+// A product's result is written to its registers 12 (32x32) or 8 (16x16) wait states after its last instruction was issued. The
+// compiler keeps what it emits away from them for so long, but does not look into inline assembly: values that max3 takes
+// from a product pass through here first.
+__device__ __forceinline__ void settle(f32x16& s) { asm("s_nop 11" : "+v"(s)); }
+__device__ __forceinline__ void settle(f32x16& s, f32x16& t) { asm("s_nop 11" : "+v"(s), "+v"(t)); }
+__device__ __forceinline__ void settle(f32x4& s, f32x4& t) { asm("s_nop 7" : "+v"(s), "+v"(t)); }
 // The largest of three (a NaN loses); fmaxf costs an instruction per operand more, to quiet signalling NaNs.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -487,6 +493,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[u][i] += lo[i];
     }
+    if constexpr (!kSplit) settle(s[0], s[1]);
     const uint32_t held = static_cast<uint32_t>(__ballot(slot >= 0));
 #pragma unroll
     for (int i = 0; i < kVld; ++i) {
@@ -691,6 +698,8 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
         s[n] = mfma32(ka[n][t], qv[t], s[n]);
       }
     }
+    if constexpr (NB == 2) settle(s[0], s[NB - 1]);
+    else settle(s[0]);
     if ((NB == 2 ? held != ~uint64_t{0} : static_cast<uint32_t>(held) != 0xffffffffu) || kb + 32 * NB > least) {
 #pragma unroll
       for (int n = 0; n < NB; ++n)
