@@ -349,6 +349,16 @@ __device__ __forceinline__ float add_pair(uint32_t w, float s) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(C2, w), __builtin_bit_cast(C2, 0x3f803f80u), s, false);
 }
 
+// A weight is exp2(score - (maximum - kOffset)), the maximum being that of the last rescaling, which comes where it has grown by more
+// than kGrow. fp16 has 2^-24 for its smallest step, and what a weight loses there the sum of the weights still has: with
+// weights up to 1 a key 17.4 (natural units) above 16384 others took their 4.5e-4 of the result with it. With the largest one between 2^12
+// and 2^14 a weight is off by 2^-37 of it, and fp16's range (2^16) still holds what the rounding of scores up to 10^7 adds. bf16 has the
+// exponents of fp32.
+template <int CT>
+constexpr float kOffset = CT == Q4_F16 ? 12.0f : 0.0f;
+template <int CT>
+constexpr float kGrow = CT == Q4_F16 ? 2.0f : 8.0f;
+
 // Eight softmax weights as the B operand of P V: two fp16 terms with fp32 activations, else rounded to the cache's type; the
 // sum is that of what is multiplied, so that a row's weights add to 1.
 template <int QT, int CT>
@@ -518,8 +528,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     float mb = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]),
                     max3(s[1][2], s[1][3], s[1][3]));
     mb = swap_combine32<true>(swap_combine16<true>(mb)) * a.cs;
-    // the sums are rescaled only where a maximum has grown by more than 2^8: weights stay below that
-    if (__any(mb > m + 8.0f)) {
+    if (__any(mb > m + kGrow<CT>)) {
       const float m_new = fmaxf(m, mb);
       const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
@@ -529,7 +538,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
     }
-    const float mu = m == -INFINITY ? 0.0f : m;
+    const float mu = m == -INFINITY ? 0.0f : m - kOffset<CT>;
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], a.cs, -mu));
@@ -718,7 +727,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
       mb = max3(x, y, z);
     }
     mb = swap_combine32<true>(mb) * a.cs;
-    if (__any(mb > m + 8.0f)) {
+    if (__any(mb > m + kGrow<CT>)) {
       const float m_new = fmaxf(m, mb);
       const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
@@ -728,7 +737,7 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
     }
-    const float mu = m == -INFINITY ? 0.0f : m;
+    const float mu = m == -INFINITY ? 0.0f : m - kOffset<CT>;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll

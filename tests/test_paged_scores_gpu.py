@@ -74,3 +74,21 @@ def test_scores_that_grow_along_the_keys(dev, dt, hd, rows, g):
     # scores: the exponent's factor and product are rounded, twice 2^-24 of the largest score each for a weight and the sum; a weight
     # and the sum of weights are rounded, exp2 and the sums over n keys in fp32
     line.check((2 * line.most * 2.0 ** -22 + 2 * weight_step(dt) + (n + 40) * U, 0.0))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,g", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("above", [14.0, 16.0, 17.375, 18.0, 22.0])
+def test_one_key_far_above_the_others(dev, dt, rows, g, above):
+    """The first key draws most of the attention and has the value 0 in even dims: what is left there is the share of 16384 others,
+    each far below a weight of 1."""
+    n, n_kv, hd = 16385, 8, 64
+    gen = torch.Generator().manual_seed(rows)
+    v = torch.randn(n, n_kv, hd, generator=gen)
+    v[..., ::2] = 1 + 0.125 * torch.rand(n, n_kv, hd // 2, generator=gen)
+    v[0, :, ::2] = 0
+    scores = 0.05 * torch.rand(n, generator=gen)
+    scores[0] = above
+    line = Line(dev, dt, scores, v, 64, rows, g)
+    # as above; and with an fp16 cache a weight is off by 2^-25, half of fp16's smallest step, where the largest one is 2^12 or more
+    line.check((2 * line.most * 2.0 ** -22 + 2 * weight_step(dt) + (n + 40) * U, 0.0 if dt == torch.bfloat16 else n * 2.0 ** -37))
