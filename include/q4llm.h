@@ -359,8 +359,8 @@ int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int b
  * (device int32 [ceil(shared_len / page_size)]) for every sequence, and page_table is read for the others
  * only: the shared keys are read and multiplied once for the whole batch. shared_len 0: shared_pages unused.
  * dtype (of q and out): F32 or F16 with an F16 cache, BF16 with a BF16 cache; F32 keeps fp32-level
- * accuracy (q and the softmax weights run as two fp16 terms: |q| < 65504, and a value of q is off by up to 2^-25), the
- * others round the weights to their own type. With an F16 cache a weight is off by up to 2^-37 of the largest, and
+ * accuracy (q runs as two fp16 terms: |q| < 65504, and a value of it is off by up to 2^-25). The softmax weights run as
+ * two terms of the cache's type; with an F16 cache a weight is off by up to 2^-37 of the largest, and
  * |scale q . k| < 10^7. Sums, maxima and partial results are fp32; the result does not depend on timing.
  * Rows of the cache that hold no key of a sequence may hold anything; the values of keys 0 .. seq_lens - 1 and of the
  * shared keys are finite, also those that a token does not see (a NaN there can reach tokens before it). q_row and

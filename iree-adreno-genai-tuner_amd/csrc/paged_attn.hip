@@ -52,7 +52,6 @@ __device__ __forceinline__ short4v read_tr4(const void* p) {
 // compiler keeps what it emits away from them for so long, but does not look into inline assembly: values that max3 takes
 // from a product pass through here first.
 __device__ __forceinline__ void settle(f32x16& s) { asm("s_nop 11" : "+v"(s)); }
-__device__ __forceinline__ void settle(f32x16& s, f32x16& t) { asm("s_nop 11" : "+v"(s), "+v"(t)); }
 __device__ __forceinline__ void settle(f32x4& s, f32x4& t) { asm("s_nop 7" : "+v"(s), "+v"(t)); }
 // The largest of three (a NaN loses); fmaxf costs an instruction per operand more, to quiet signalling NaNs.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -339,16 +338,6 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const Row& w, int d, v
   }
 }
 
-// s + a + b of the two 16-bit values of w, in fp32.
-template <int CT>
-__device__ __forceinline__ float add_pair(uint32_t w, float s) {
-  typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
-  if constexpr (CT == Q4_F16)
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(C2, w), __builtin_bit_cast(C2, 0x3c003c00u), s, false);
-  else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(C2, w), __builtin_bit_cast(C2, 0x3f803f80u), s, false);
-}
-
 // A weight is exp2(score - (maximum - kOffset)), the maximum being that of the last rescaling, which comes where it has grown by more
 // than kGrow. fp16 has 2^-24 for its smallest step, and what a weight loses there the sum of the weights still has: with
 // weights up to 1 a key 17.4 (natural units) above 16384 others took their 4.5e-4 of the result with it. With the largest one between 2^12
@@ -359,31 +348,32 @@ constexpr float kOffset = CT == Q4_F16 ? 12.0f : 0.0f;
 template <int CT>
 constexpr float kGrow = CT == Q4_F16 ? 2.0f : 8.0f;
 
-// Eight softmax weights as the B operand of P V: two fp16 terms with fp32 activations, else rounded to the cache's type; the
-// sum is that of what is multiplied, so that a row's weights add to 1.
-template <int QT, int CT>
-__device__ __forceinline__ void weights8(const float (&p)[8], float neg1, vec8<CT>* hi_out, vec8<CT>* lo_out, float* sum) {
-  typedef vec8<CT> C8;
-  if constexpr (QT == Q4_F32) {
-    uint32_t hi[4], lo[4];
+// Eight softmax weights as the B operand of P V, in two terms of the cache's type that are multiplied one after the other: the weights
+// rounded, and what that leaves. One term alone put the results of fp16 and bf16 activations 1.35 times as far from the exact ones
+// as their own rounding does; two cost a third of the matrix products more (prompts behind 4096 shared keys 190 -> 239 us, 5 drafted tokens
+// each of 48 sequences 53 -> 61, single tokens up to 3%). The second term is formed while the first one's products run.
+template <int CT>
+__device__ __forceinline__ vec8<CT> upper8(const float (&p)[8]) {
+  typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split_f16_pair(p[2 * i], p[2 * i + 1], neg1, hi[i], lo[i]);
-    *hi_out = __builtin_bit_cast(C8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-    *lo_out = __builtin_bit_cast(C8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{p[2 * i], p[2 * i + 1]}), C2));
+  return __builtin_bit_cast(vec8<CT>, make_uint4(w[0], w[1], w[2], w[3]));
+}
+template <int CT>
+__device__ __forceinline__ vec8<CT> lower8(const float (&p)[8], vec8<CT> upper, float neg1) {
+  const uint4 u4 = __builtin_bit_cast(uint4, upper);
+  const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w};
+  float left[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *sum += p[i];
-  } else {
-    typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const C2 r = __builtin_convertvector((f32x2{p[2 * i], p[2 * i + 1]}), C2);
-      w[i] = __builtin_bit_cast(uint32_t, r);
-      *sum = add_pair<CT>(w[i], *sum);
-    }
-    *hi_out = __builtin_bit_cast(C8, make_uint4(w[0], w[1], w[2], w[3]));
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (CT == Q4_F16)
+      left[i] = fmaf(static_cast<float>(upper[i]), neg1, p[i]);  // one instruction that reads the half as it is
+    else
+      left[i] = p[i] - __builtin_bit_cast(float, i & 1 ? u[i / 2] & 0xffff0000u : u[i / 2] << 16);
   }
+  return upper8<CT>(left);
 }
 
 // N consecutive values of a range's o; or of the result, where it is the only range of the row.
@@ -424,7 +414,7 @@ template <int QT, int CT, int HD>
 __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, int entry, unsigned char* buf0,
                                              unsigned char* buf1, float2 (*wml)[64]) {
   typedef vec8<CT> C8;
-  constexpr bool kSplit = QT == Q4_F32;      // q and P as two fp16 terms
+  constexpr bool kSplit = QT == Q4_F32;      // q as two fp16 terms
   constexpr int KS = HD / 32, OT = HD / 16;  // MFMA steps over the dims; 16-dim output tiles
   constexpr int kRowB = HD * 2;
   constexpr int kCpr = HD / 8;               // 16-byte chunks per row
@@ -515,7 +505,6 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     slot = slot_of(entry, kb + it.step);
     if (kb + it.step < k1) load(slot);
     entry = page_entry(kb + 2 * it.step);
-    C8 ph, pl;
     if (held != 0xffffffffu || kb + kKeys > least) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -542,7 +531,9 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], a.cs, -mu));
-    weights8<QT, CT>(p, neg1, &ph, &pl, &l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l += p[i];
+    const C8 ph = upper8<CT>(p), pl = lower8<CT>(p, ph, neg1);
 #pragma unroll
     for (int d = 0; d < OT; ++d) {
       short4v v[2];
@@ -553,7 +544,7 @@ __device__ __forceinline__ void paged_stream(const AttnArgs& a, const Item& it, 
       }
       const C8 va = __builtin_bit_cast(C8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
       o[d] = mfma16(va, ph, o[d]);
-      if constexpr (kSplit) o[d] = mfma16(va, pl, o[d]);
+      o[d] = mfma16(va, pl, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -622,7 +613,6 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
   typedef vec8<CT> C8;
   constexpr bool kSplit = QT == Q4_F32;
   constexpr int KW = kWaves / RW;
-  constexpr int NB = KW == 1 && !kSplit ? 2 : 1;  // 32-key blocks of a wave at once (two terms: registers for one)
   constexpr int KS = HD / 16, OT = HD / 32;       // MFMA steps over the dims; 32-dim output tiles
   constexpr int kRowB = HD * 2;
   constexpr int kCpr = HD / 8;
@@ -686,47 +676,34 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
 #pragma unroll
   for (int d = 0; d < OT; ++d) vcol[d] = vrow + (((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz<HD>(kr4)) << 4);
 
-  // NB blocks from key row r0 of a stage on; kb: the first one's first key.
-  auto compute = [&](const unsigned char* buf, int r0, int kb, uint64_t held) __attribute__((always_inline)) {
+  // The block of 32 keys from row r0 of a stage on; kb: its first key. (Two blocks at a time, as far as the registers hold them: prompts
+  // 240 instead of 238 us.)
+  auto compute = [&](const unsigned char* buf, int r0, int kb, uint32_t held) __attribute__((always_inline)) {
     if (kb >= most) return;
     const unsigned char* Ks = buf + r0 * kRowB;
     const unsigned char* Vs = Ks + kHalf;
-    f32x16 s[NB];
-    C8 ka[NB][KS];
+    C8 ka[KS];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int t = 0; t < KS; ++t)
+      ka[t] = *reinterpret_cast<const C8*>(Ks + ql_ * kRowB + (((2 * t + half) ^ kswz<HD>(ql_)) << 4));
+    f32x16 s = {};
 #pragma unroll
-      for (int t = 0; t < KS; ++t)
-        ka[n][t] = *reinterpret_cast<const C8*>(Ks + (32 * n + ql_) * kRowB + (((2 * t + half) ^ kswz<HD>(ql_)) << 4));
+    for (int t = 0; t < KS; ++t) {
+      if constexpr (kSplit) s = mfma32(ka[t], qlo[t], s);
+      s = mfma32(ka[t], qv[t], s);
+    }
+    settle(s);
+    if (held != 0xffffffffu || kb + 32 > least) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      s[n] = f32x16{};
-#pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        if constexpr (kSplit) s[n] = mfma32(ka[n][t], qlo[t], s[n]);
-        s[n] = mfma32(ka[n][t], qv[t], s[n]);
+      for (int e = 0; e < 16; ++e) {
+        const int k = 8 * (e >> 2) + 4 * half + (e & 3);
+        if (kb + k >= w.lim || !((held >> k) & 1)) s[e] = -INFINITY;
       }
     }
-    if constexpr (NB == 2) settle(s[0], s[NB - 1]);
-    else settle(s[0]);
-    if ((NB == 2 ? held != ~uint64_t{0} : static_cast<uint32_t>(held) != 0xffffffffu) || kb + 32 * NB > least) {
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 32 * n + 8 * (e >> 2) + 4 * half + (e & 3);
-          if (kb + k >= w.lim || !((held >> k) & 1)) s[n][e] = -INFINITY;
-        }
-    }
-    float mb = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const float x = max3(max3(s[n][0], s[n][1], s[n][2]), s[n][3], s[n][4]);
-      const float y = max3(max3(s[n][5], s[n][6], s[n][7]), s[n][8], s[n][9]);
-      const float z = max3(max3(s[n][10], s[n][11], s[n][12]), max3(s[n][13], s[n][14], s[n][15]), mb);
-      mb = max3(x, y, z);
-    }
-    mb = swap_combine32<true>(mb) * a.cs;
+    const float x = max3(max3(s[0], s[1], s[2]), s[3], s[4]);
+    const float y = max3(max3(s[5], s[6], s[7]), s[8], s[9]);
+    const float z = max3(max3(s[10], s[11], s[12]), max3(s[13], s[14], s[15]), -INFINITY);
+    const float mb = swap_combine32<true>(max3(x, y, z)) * a.cs;
     if (__any(mb > m + kGrow<CT>)) {
       const float m_new = fmaxf(m, mb);
       const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
@@ -739,27 +716,26 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
     }
     const float mu = m == -INFINITY ? 0.0f : m - kOffset<CT>;
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int u = 0; u < 2; ++u) {
+      float p[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[8];
+      for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], a.cs, -mu));
+      const C8 ph = upper8<CT>(p);
+      C8 va[OT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[n][8 * u + i], a.cs, -mu));
-        C8 ph, pl;
-        weights8<QT, CT>(p, neg1, &ph, &pl, &l);
-        C8 va[OT];
-#pragma unroll
-        for (int d = 0; d < OT; ++d) {
-          const short4v v0 = read_tr4(Vs + vcol[d] + (32 * n + 16 * u) * kRowB);
-          const short4v v1 = read_tr4(Vs + vcol[d] + (32 * n + 16 * u + 8) * kRowB);
-          va[d] = __builtin_bit_cast(C8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-#pragma unroll
-        for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], ph, o[d]);
-        if constexpr (kSplit)
-#pragma unroll
-          for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], pl, o[d]);
+      for (int d = 0; d < OT; ++d) {
+        const short4v v0 = read_tr4(Vs + vcol[d] + 16 * u * kRowB);
+        const short4v v1 = read_tr4(Vs + vcol[d] + (16 * u + 8) * kRowB);
+        va[d] = __builtin_bit_cast(C8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
       }
+#pragma unroll
+      for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], ph, o[d]);
+      const C8 pl = lower8<CT>(p, ph, neg1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l += p[i];
+#pragma unroll
+      for (int d = 0; d < OT; ++d) o[d] = mfma32(va[d], pl, o[d]);
+    }
   };
 
   // All loads of this wave have landed and its reads are done; then all waves'.
@@ -786,12 +762,10 @@ __device__ __forceinline__ void paged_shared(const AttnArgs& a, const Item& it, 
       entry = page_entry(kb + 2 * it.step);
       held = __ballot(slot >= 0);
       if constexpr (KW == 2) {
-        compute(cur, 32 * kw, kb + 32 * kw, now >> (32 * kw));
-      } else if constexpr (NB == 2) {
-        compute(cur, 0, kb, now);
+        compute(cur, 32 * kw, kb + 32 * kw, static_cast<uint32_t>(now >> (32 * kw)));
       } else {
-        compute(cur, 0, kb, now);
-        compute(cur, 32, kb + 32, now >> 32);
+        compute(cur, 0, kb, static_cast<uint32_t>(now));
+        compute(cur, 32, kb + 32, static_cast<uint32_t>(now >> 32));
       }
       kb += it.step;
       turn();
