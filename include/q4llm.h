@@ -357,7 +357,8 @@ int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int b
  * their sequences' keys: token at position p sees keys 0 .. p below L and below its sequence's length; o =
  * softmax(scale q . k) . v, zeros where it sees none. Keys 0 .. shared_len - 1 are taken from shared_pages
  * (device int32 [ceil(shared_len / page_size)]) for every sequence, and page_table is read for the others
- * only: the shared keys are read and multiplied once for the whole batch. shared_len 0: shared_pages unused.
+ * only (its rows may be shorter than the prefix): the shared keys are read and multiplied once for the whole batch.
+ * shared_len 0: shared_pages unused.
  * dtype (of q and out): F32 or F16 with an F16 cache, BF16 with a BF16 cache; F32 keeps fp32-level
  * accuracy (q runs as two fp16 terms: |q| < 65504, and a value of it is off by up to 2^-25). The softmax weights run as
  * two terms of the cache's type; with an F16 cache a weight is off by up to 2^-37 of the largest, and

@@ -72,6 +72,7 @@ struct AttnArgs {
   int2* own;  // null: every row has one range
   const int32_t* shared_pages;
   int T, n_q, n_kv, g, L, shared_len;
+  int held;  // keys that the page lists hold, the shared ones or those of page_table (which the prefix may exceed), L at most
   int shared_blocks, shared_splits, shared_tile;  // workgroups of the shared ranges, ranges, rows of a workgroup
   int own_from, slot_rows, own_rows;              // own ranges: their first key, rows of a slot and of all slots
   bool longest_first, refill;
@@ -297,7 +298,8 @@ __device__ __forceinline__ Row row_of(const AttnArgs& a, const Item& it, int r) 
     if (w.ok && s < a.b.batch) {
       const int2 tk = tokens_of(a.b, s, a.T);
       w.ok = w.token >= tk.x && w.token < tk.x + tk.y;
-      w.lim = min(min(a.b.lens[s] - tk.y + (w.token - tk.x) + 1, a.b.keys_of(a.b.lens[s])), a.shared_len);
+      const int len = a.b.lens[s];
+      w.lim = min(min(len - tk.y + (w.token - tk.x) + 1, max(len, 0)), a.shared_len);
     } else {
       w.ok = false;
     }
@@ -861,7 +863,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
   it.k1 = a.shared_len;
   if (!it.shared) {
     const int len = a.b.lens[it.seq], tokens = a.b.cu ? it.n_rows / a.g : a.b.rows;
-    it.own_end = min(a.b.keys_of(len), a.L);
+    it.own_end = min(max(len, 0), a.held);
     it.behind = len - tokens;
     // no row of the tile sees more than its last
     const int last = a.by_g.div(min(it.row0 + height, it.n_rows) - 1);
@@ -1122,6 +1124,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
   a.shared_pages = shared_pages;
   a.T = static_cast<int>(T), a.n_q = n_q, a.n_kv = kv->n_kv, a.g = g, a.L = L, a.shared_len = shared_len;
   a.shared_blocks = static_cast<int>(p.shared_blocks), a.shared_splits = p.shared_splits, a.shared_tile = p.shared_tile;
+  a.held = static_cast<int>(std::min<int64_t>(std::max<int64_t>(int64_t{kv->max_pages} * kv->page_size, shared_len), L));
   a.own_from = p.own_from, a.slot_rows = p.slot_rows;
   a.longest_first = p.longest_first, a.refill = p.refill, a.turn_from = p.turn_from;
   // a negative scale turns q around and a zero one clears it, so that the exponents' factor is positive

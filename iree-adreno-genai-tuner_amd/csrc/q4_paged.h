@@ -48,11 +48,6 @@ struct PagedBatch {
   int rows;  // tokens of each sequence where cu is null
   FastDiv by_rows, by_page;
 
-  // The keys of a sequence of length n that its page list can hold.
-  __device__ __forceinline__ int keys_of(int n) const {
-    const int64_t most = static_cast<int64_t>(max_pages) * page_size;
-    return static_cast<int>(min(static_cast<int64_t>(max(n, 0)), most));
-  }
   // Row of the cache that entry `page` of a page list gives at offset `off`, -1 for no page of the pool.
   __device__ __forceinline__ int slot(int page, int off) const {
     return page >= 0 && page < num_pages ? page * page_size + off : -1;

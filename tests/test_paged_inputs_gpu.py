@@ -3,11 +3,39 @@
 import pytest
 import torch
 
-from test_paged_gpu import Batch, half_step
+from test_paged_gpu import DTYPES, IDS, Batch, check_rounded, half_step
 
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shared,cols", [(100, 1), (100, 6), (640, 1), (640, 39)])
+@pytest.mark.parametrize("rows,ragged", [([1] * 6, False), ([5] * 6, False), ([1, 7, 140, 2, 3, 9], True)])
+def test_a_page_table_narrower_than_the_prefix(dev, dt, shared, cols, rows, ragged):
+    """Keys of the prefix come from shared_pages, whatever page_table holds; the keys behind it have no page here."""
+    page, hd = 16, 64
+    lens = [shared, shared - 3, shared + 9, 20, shared, shared + 400]
+    b = Batch(dev, dt, hd, 2, page, lens, rows, shared, ragged, seed=shared + cols)
+    b.page_table = torch.full((6, cols), 1 << 20, dtype=torch.int32, device=dev)  # no page of the pool
+    b.check(b.q(6), hd ** -0.5, L=shared)  # (reference: no key from `shared` on)
+    got = b.attn(b.q(6), hd ** -0.5, L=shared + 512)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shared", [100, 640])
+def test_a_page_table_wider_than_the_prefix_ends_before_the_keys(dev, dt, shared):
+    """Positions from max_pages * page_size on have no page: the keys before them are all there are."""
+    page, hd, cols = 16, 64, shared // 16 + 2
+    lens = [shared + 200, shared + 3, shared + 40, shared]
+    b = Batch(dev, dt, hd, 2, page, lens, [1] * 4, shared, seed=shared)
+    b.page_table = b.page_table[:, :cols].contiguous()
+    q = b.q(6)
+    ref, err = b.reference(q, hd ** -0.5, L=cols * page)
+    got = b.attn(q, hd ** -0.5, L=max(lens))
+    check_rounded(got.unflatten(1, (6, hd)), ref, err, dt)
 
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
