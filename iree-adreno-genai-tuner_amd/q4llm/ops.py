@@ -591,7 +591,7 @@ def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shar
     dev = _same_device(q, k_cache, v_cache, page_table, seq_lens, cu_q, shared_pages if shared_len else None, workspace, out)
     align = 16 // q.element_size()
     if q.stride(0) % align or q.stride(1) % align or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)  # (contiguous() leaves a start off 16 bytes, and strides of single rows)
     if L is None:
         L = min(max(kv.max_pages * kv.page_size, shared_len), 1 << 30)
     need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len)

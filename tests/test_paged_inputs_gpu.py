@@ -38,6 +38,27 @@ def test_a_page_table_wider_than_the_prefix_ends_before_the_keys(dev, dt, shared
     check_rounded(got.unflatten(1, (6, hd)), ref, err, dt)
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_queries_off_16_bytes_and_strides_of_single_rows(dev, dt):
+    """q that starts between 16-byte words, and q whose one token or one head has a stride that is no multiple of 16 bytes: the same
+    bits as an aligned copy of it gives."""
+    hd = 64
+    one = Batch(dev, dt, hd, 1, 16, [70], [1], seed=1)
+    more = Batch(dev, dt, hd, 1, 16, [70, 33], [2, 2], seed=2)
+    for b, n_q in ((one, 1), (one, 3), (more, 1), (more, 4)):
+        q = b.q(n_q)
+        want = b.check(q, hd ** -0.5)
+        t = q.shape[0]
+        flat = torch.zeros(q.numel() + 8, dtype=dt, device=dev)
+        flat[1:1 + q.numel()] = q.flatten()
+        shifted = flat[1:1 + q.numel()].view(t, n_q, hd)
+        odd = torch.zeros(2 * q.numel() + 64, dtype=dt, device=dev)
+        strides = (n_q * hd if t > 1 else 1, hd if n_q > 1 else 3, 1)
+        strided = odd.as_strided(q.shape, strides).copy_(q)
+        for x in (shifted, strided):
+            assert torch.equal(b.attn(x, hd ** -0.5), want)
+
+
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows,lens,shared", [([1, 1, 1], [9, 30, 17], 0), ([12, 5, 17], [12, 30, 17], 0), ([150, 90, 3], [150, 95, 40], 0),
