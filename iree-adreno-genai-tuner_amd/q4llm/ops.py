@@ -594,6 +594,8 @@ def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shar
         q = q.clone(memory_format=torch.contiguous_format)  # (contiguous() leaves a start off 16 bytes, and strides of single rows)
     if L is None:
         L = min(max(kv.max_pages * kv.page_size, shared_len), 1 << 30)
+    if t == kv.batch == 0:
+        return torch.empty(0, n_q * hd, dtype=q.dtype, device=dev) if out is None else out
     need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len)
     if workspace is None:
         workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from q4llm import ops
 from test_paged_gpu import DTYPES, IDS, Batch, check_rounded, half_step
 
 pytestmark = pytest.mark.gpu
@@ -57,6 +58,23 @@ def test_queries_off_16_bytes_and_strides_of_single_rows(dev, dt):
         strided = odd.as_strided(q.shape, strides).copy_(q)
         for x in (shifted, strided):
             assert torch.equal(b.attn(x, hd ** -0.5), want)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+def test_no_sequence_and_no_token(dev, dt):
+    hd = 64
+    k = torch.zeros(3, 16, 2, hd, dtype=torch.bfloat16 if dt == torch.bfloat16 else torch.float16, device=dev)
+    q = torch.zeros(0, 4, hd, dtype=dt, device=dev)
+    for batch in (0, 2):
+        table, lens = torch.zeros(batch, 4, dtype=torch.int32, device=dev), torch.zeros(batch, dtype=torch.int32, device=dev)
+        assert ops.paged_attn(q, k, k.clone(), table, lens, 0.125).shape == (0, 4 * hd)
+        assert ops.paged_kv_append(q[:, :2], q[:, :2], k, k.clone(), table, lens, q=q).shape == (0, 4, hd)
+    assert ops.rope_rotate(q, lens[:0], ops_rope(dev)).shape == (0, 4, hd)
+
+
+def ops_rope(dev):
+    from q4llm.rope import Rope
+    return Rope(torch.ones(16, device=dev))
 
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
