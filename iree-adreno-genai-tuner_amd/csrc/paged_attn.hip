@@ -980,6 +980,7 @@ struct Plan {
 
 Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int shared_len) {
   Plan p{};
+  if (T == 0) return p;
   const int g = n_q / n_kv;
   const int64_t rows = T * g;
   // The shared keys are a range of their own where that saves reading them once for each sequence: not for one sequence, not
