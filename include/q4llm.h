@@ -349,9 +349,13 @@ int paged_kv_append(const q4_paged_kv* kv, const void* k, int64_t k_row, int64_t
                     int64_t q_head, void* q_out, int64_t qo_row, int64_t qo_head, int n_q, void* stream);
 
 /* Workspace bytes of paged_attn for T tokens, n_q heads, a batch of `batch` sequences with at most L keys, the first
- * shared_len of them shared. */
+ * shared_len of them shared: enough with kv->cu_q and without it. The _for form is that of one of the two: has_cu_q nonzero or 0
+ * (without, the rows of every sequence are known and need far less, often nothing). Both are for calls with these very numbers:
+ * one with fewer tokens or keys can need more. */
 int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
                                size_t* bytes);
+int paged_attn_workspace_bytes_for(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
+                                   int has_cu_q, size_t* bytes);
 
 /* Causal GQA attention of the T tokens of a step (q: T x n_q x head_dim, rotated; out: [T, n_q * head_dim]) over
  * their sequences' keys: token at position p sees keys 0 .. p below L and below its sequence's length; o =

@@ -1078,16 +1078,21 @@ int launch(const AttnArgs& a, int64_t blocks, int most, hipStream_t st) {
 
 using namespace q4;
 
-extern "C" int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
-                                          size_t* bytes) {
+extern "C" int paged_attn_workspace_bytes_for(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
+                                              int has_cu_q, size_t* bytes) {
   if (!bytes) return Q4_ERR_NULL;
   if (int st = attn_args(T, n_q, n_kv, head_dim, batch, L, shared_len)) return st;
-  size_t most = 0;
-  for (const bool ragged : {false, true}) {  // with cu_q or not
-    if (!ragged && T % batch) continue;
-    most = std::max(most, workspace_of(plan_for(T, n_q, n_kv, batch, ragged, L, shared_len), T * n_q, head_dim));
-  }
-  *bytes = most;
+  if (!has_cu_q && T % batch) return Q4_ERR_SHAPE;
+  *bytes = workspace_of(plan_for(T, n_q, n_kv, batch, has_cu_q != 0, L, shared_len), T * n_q, head_dim);
+  return Q4_OK;
+}
+
+extern "C" int paged_attn_workspace_bytes(int64_t T, int n_q, int n_kv, int head_dim, int batch, int L, int shared_len,
+                                          size_t* bytes) {
+  if (int st = paged_attn_workspace_bytes_for(T, n_q, n_kv, head_dim, batch, L, shared_len, 1, bytes)) return st;
+  size_t even = 0;
+  if (T % batch == 0) paged_attn_workspace_bytes_for(T, n_q, n_kv, head_dim, batch, L, shared_len, 0, &even);
+  *bytes = std::max(*bytes, even);
   return Q4_OK;
 }
 

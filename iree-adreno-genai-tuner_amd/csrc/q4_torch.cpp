@@ -380,8 +380,8 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const c10::DeviceGuard on(q.device());
     if (!ws.defined()) {
       size_t need = 0;
-      if (paged_attn_workspace_bytes(t, static_cast<int>(n_q), p.kv.n_kv, static_cast<int>(hd), p.kv.batch,
-                                     static_cast<int>(L), static_cast<int>(shared), &need) != Q4_OK)
+      if (paged_attn_workspace_bytes_for(t, static_cast<int>(n_q), p.kv.n_kv, static_cast<int>(hd), p.kv.batch,
+                                         static_cast<int>(L), static_cast<int>(shared), p.cu.defined(), &need) != Q4_OK)
         Py_RETURN_NONE;
       ws = at::empty({static_cast<int64_t>(std::max<size_t>(need, 16))}, q.options().dtype(at::kByte));
     }

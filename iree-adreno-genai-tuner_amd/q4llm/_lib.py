@@ -67,6 +67,7 @@ SIGNATURES = {
     "rope_rotate": [p, i64, i64, p, i64, i64, i32, i64, i32, i32, p, p, i32, p],
     "paged_kv_append": [p, p, i64, i64, p, i64, i64, i32, i64, p, p, i64, i64, p, i64, i64, i32, p],
     "paged_attn_workspace_bytes": [i64, i32, i32, i32, i32, i32, i32, C.POINTER(sz)],
+    "paged_attn_workspace_bytes_for": [i64, i32, i32, i32, i32, i32, i32, i32, C.POINTER(sz)],
     "paged_attn": [p, p, i64, i64, p, i32, i64, i32, i32, p, i32, f32, p, sz, p],
     "spec_verify_workspace_bytes": [i32, i32, i64, C.POINTER(sz)],
     "spec_verify": [p, i64, p, i64, i64, p, i64, i64, p, i64, p, i32, i32, i64, p, p, p, sz, p],

@@ -559,9 +559,13 @@ def paged_kv_append(k, v, k_cache, v_cache, page_table, seq_lens, cu_q=None, rop
     return q_out
 
 
-def paged_attn_workspace_bytes(T, n_q, n_kv, hd, batch, L, shared_len=0) -> int:
+def paged_attn_workspace_bytes(T, n_q, n_kv, hd, batch, L, shared_len=0, ragged=None) -> int:
+    """ragged: of calls with cu_q, or (False) without, which need far less; None: enough for both."""
     b = C.c_size_t(0)
-    LIB.call("paged_attn_workspace_bytes", T, n_q, n_kv, hd, batch, L, shared_len, C.byref(b))
+    if ragged is None:
+        LIB.call("paged_attn_workspace_bytes", T, n_q, n_kv, hd, batch, L, shared_len, C.byref(b))
+    else:
+        LIB.call("paged_attn_workspace_bytes_for", T, n_q, n_kv, hd, batch, L, shared_len, int(ragged), C.byref(b))
     return b.value
 
 
@@ -596,7 +600,7 @@ def paged_attn(q, k_cache, v_cache, page_table, seq_lens, scale, cu_q=None, shar
         L = min(max(kv.max_pages * kv.page_size, shared_len), 1 << 30)
     if t == kv.batch == 0:
         return torch.empty(0, n_q * hd, dtype=q.dtype, device=dev) if out is None else out
-    need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len)
+    need = paged_attn_workspace_bytes(t, n_q, kv.n_kv, hd, kv.batch, L, shared_len, cu_q is not None)
     if workspace is None:
         workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
     if out is None:

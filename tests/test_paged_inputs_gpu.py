@@ -104,3 +104,20 @@ def test_16_bit_weights_are_as_exact_as_sums_in_32_bits(dev, dt, hd, rows, lens,
             worst = ((got[at] - ref[at]).abs() / tol).max().item()
             assert worst <= 1, (s, i, worst)
             at += 1
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_the_wrapper_takes_the_workspace_of_its_own_form(dev, ragged):
+    """Nothing beside the result for 64 single tokens of at most 1000 keys without cu_q; and that query's bytes are enough."""
+    n, n_q, n_kv, hd, L = 64, 24, 8, 128, 1000
+    b = Batch(dev, torch.float16, hd, n_kv, 16, [1 + 2 * i for i in range(n)], [1] * n, 0, ragged)
+    q = b.q(n_q)
+    need = ops.paged_attn_workspace_bytes(n, n_q, n_kv, hd, n, L, 0, ragged)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = b.check(q, hd ** -0.5, L=L)
+    assert torch.cuda.max_memory_allocated() - before <= max(need, 16) + out.numel() * 2 + 4096
+    assert (need == 0) == (not ragged)
+    ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device=dev)
+    assert torch.equal(b.attn(q, hd ** -0.5, L=L, workspace=ws), out)
