@@ -294,7 +294,8 @@ int argmax_f32(const float* logits, int64_t V, int32_t* out, void* workspace, si
  * Batched serving over a paged KV cache (no counterpart in the reference, which steps one sequence
  * over a dense cache): rotary positions, the write of new keys and values, attention with a prefix
  * that the batch shares, and the check of drafted tokens. Every length, position and page is read
- * on the device, so a captured call serves later steps with the same sizes.
+ * on the device, so a captured call serves later steps with the same sizes. Sizes past those of one launch (2^24 workgroups;
+ * about as many tokens, or 2^27 rows of tokens and heads) are refused with Q4_ERR_SHAPE before anything is launched.
  * ------------------------------------------------------------------------------------------- */
 
 /* Which dims of the rotated part of a head form a pair: (i, i + rot_dim / 2) or (2i, 2i + 1). */

@@ -1059,14 +1059,15 @@ int attn_args(int64_t T, int n_q, int n_kv, int hd, int batch, int L, int shared
 
 template <int QT, int CT, int HD>
 int launch(const AttnArgs& a, int64_t blocks, int most, hipStream_t st) {
+  const int64_t rows = static_cast<int64_t>(a.T) * a.n_q;
+  const int pg = most <= 4 || rows >= 16384 ? 1 : most <= 16 ? 4 : 8, per = 256 / (HD / 4 * pg);
+  if (!fits_grid(blocks, kThreads) || (most > 1 && !fits_grid((rows + per - 1) / per, 256))) return Q4_ERR_SHAPE;
   if (blocks > 0)
     hipLaunchKernelGGL((paged_attn_kernel<QT, CT, HD>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
   if (most > 1) {
-    // a few ranges a thread, so that a row is one round trip; a thread a row where there are rows enough to fill the chip.
+    // (pg) a few ranges a thread, so that a row is one round trip; a thread a row where there are rows enough to fill the chip.
     // With 1 / 4 / 8: one sequence of 700 keys 9.9 / 9.6 / 9.6 us, of 16000 30.8 / 21.8 / 20.3, 7680 rows of 5 ranges
     // 57 / 58 / 61, 65000 rows of 2 to 4 ranges 191 / 204 / 218.
-    const int64_t rows = static_cast<int64_t>(a.T) * a.n_q;
-    const int pg = most <= 4 || rows >= 16384 ? 1 : most <= 16 ? 4 : 8, per = 256 / (HD / 4 * pg);
     const auto fn = pg == 1 ? paged_join_kernel<QT, HD, 1> : pg == 4 ? paged_join_kernel<QT, HD, 4> : paged_join_kernel<QT, HD, 8>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st, a);
   }
@@ -1118,7 +1119,7 @@ extern "C" int paged_attn(const q4_paged_kv* kv, const void* q, int64_t q_row, i
     if (!aligned(workspace, 16)) return Q4_ERR_ALIGN;
   }
   const int64_t blocks = p.shared_blocks + p.own_blocks;
-  if (blocks > INT32_MAX || p.partials > INT32_MAX) return Q4_ERR_SHAPE;
+  if (p.partials > INT32_MAX) return Q4_ERR_SHAPE;
   a.q = q, a.qr = q_row, a.qh = q_head;
   a.kc = kv->k_cache, a.vc = kv->v_cache, a.out = out;
   if (p.partials) {

@@ -27,6 +27,9 @@ inline int launch_status() {
   return e == hipSuccess ? Q4_OK : hip_fail(e);
 }
 
+// A launch of `blocks` workgroups of `threads` threads: a queue's packet counts the threads in 32 bits.
+inline bool fits_grid(int64_t blocks, int threads) { return blocks <= UINT32_MAX / threads; }
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }

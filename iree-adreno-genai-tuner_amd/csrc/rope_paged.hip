@@ -334,6 +334,7 @@ int launch_rope(const void* x, int64_t xr, int64_t xh, void* y, int64_t yr, int6
   const int units = in_place ? U::rotated(r.half) : U::count(hd, r.half);
   if (units == 0) return Q4_OK;
   const Split s = split_for(T, heads * units, r.half);
+  if (!fits_grid((T + s.tpb - 1) / s.tpb, kThreads)) return Q4_ERR_SHAPE;
   const size_t lds = 8 * ((s.tpb + 1) / 2 + static_cast<size_t>(s.tpb) * r.half);
   const bool stream = T * heads * hd * static_cast<int64_t>(sizeof(typename U::T)) > kStream;
   const auto fn = VB == 16 && stream ? rope_kernel<DT, LAYOUT, VB, VB == 16> : rope_kernel<DT, LAYOUT, VB, false>;
@@ -354,6 +355,7 @@ template <int DT, int CT, int LAYOUT, int VB>
 int launch_append(AppendArgs& a, hipStream_t st) {
   a.units = Unit<DT, LAYOUT, VB>::count(a.hd, a.r.half);
   const Split s = split_for(a.T, a.heads * a.units, a.r.half);
+  if (!fits_grid((int64_t{a.T} + s.tpb - 1) / s.tpb, kThreads)) return Q4_ERR_SHAPE;
   a.tpb = s.tpb;
   a.part = s.part;
   a.by_units = FastDiv(a.units);
@@ -362,7 +364,7 @@ int launch_append(AppendArgs& a, hipStream_t st) {
   const size_t lds = 8 * (s.tpb + static_cast<size_t>(s.tpb) * a.r.half);
   const bool stream = static_cast<int64_t>(a.T) * a.heads * a.hd * static_cast<int64_t>(sizeof(typename Num<DT>::type)) > kStream;
   const auto fn = VB == 16 && stream ? append_kernel<DT, CT, LAYOUT, VB, VB == 16> : append_kernel<DT, CT, LAYOUT, VB, false>;
-  hipLaunchKernelGGL(fn, dim3((a.T + s.tpb - 1) / s.tpb, s.parts), dim3(kThreads), lds,
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((int64_t{a.T} + s.tpb - 1) / s.tpb), s.parts), dim3(kThreads), lds,
                      st, a);
   return launch_status();
 }

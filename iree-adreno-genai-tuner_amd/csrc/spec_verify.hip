@@ -282,7 +282,9 @@ extern "C" int spec_verify(const int32_t* tokens, int64_t tok_row, const float* 
   VerifyArgs a{tokens, draft, target, uniforms, n_draft, tok_row, draft_batch, draft_row, target_batch, target_row, uni_row,
                K, static_cast<int>(V), chunks_of(V), static_cast<double2*>(workspace), out_tokens, n_accepted};
   const hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(verify_sum_kernel, dim3(static_cast<unsigned>(B) * ((a.chunks + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
+  const int64_t sums = static_cast<int64_t>(B) * ((a.chunks + kWaves - 1) / kWaves);
+  if (!fits_grid(sums, kThreads)) return Q4_ERR_SHAPE;
+  hipLaunchKernelGGL(verify_sum_kernel, dim3(static_cast<unsigned>(sums)), dim3(kThreads), 0, st, a);
   hipLaunchKernelGGL(verify_pick_kernel, dim3(B), dim3(kThreads), 0, st, a);
   return launch_status();
 }
