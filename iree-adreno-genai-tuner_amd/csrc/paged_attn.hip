@@ -1005,7 +1005,6 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
     p.refill = rows / batch <= 32 && keys >= 2048;
     p.own_tiles = ragged ? 1 : tiles_of(rows / batch);
     const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv;
-    const int slots = p.refill ? 2 * kSlots : kSlots;
     // Short keys are one range, which needs no join: up to two blocks a wave always, up to four where there are items for a
     // quarter of the units. One token each of 1 / 4 / 12 / 32 sequences, 8 KV heads of 128, one range and as many as fit:
     // 250 keys 7.8 / 7.9 / 8.9 / 10.5 and 8.8 / 8.8 / 10.6 / 13.6 us, 400 keys 9.9 / 10.0 / 11.4 / 14.1 and 8.9 / 10.0 /
@@ -1015,7 +1014,8 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
     if (ragged) {
       // the number of tiles, and so of ranges, is known on the device alone; at most one tile that is not full a sequence, and
       // a full one has 128 rows
-      p.own_blocks = (rows / 128 + batch) * n_kv + slots;
+      const int64_t most = (rows / 128 + batch) * n_kv, fill = p.refill ? 2 * p.places : p.places;  // items; what ranges fill
+      p.own_blocks = std::max(most, (most < kSlots ? 0 : most) + fill);  // (fewer than kSlots: none is whole)
       p.slot_rows = tile_rows(rows);
     } else {
       const int64_t rest = items % kSlots;

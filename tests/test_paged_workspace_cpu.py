@@ -26,3 +26,11 @@ def test_the_query_for_one_form_refuses_what_the_call_would():
         with pytest.raises(Exception):
             ops.paged_attn_workspace_bytes(*a.values(), False)
     assert ops.paged_attn_workspace_bytes(7, 8, 2, 64, 4, 4000, 0, True) > 0  # 7 tokens of 4 sequences: with cu_q
+
+
+def test_slots_with_cu_q_are_those_that_ranges_can_fill():
+    """32 single tokens behind 2048 shared keys (8 KV heads of 128 dims): 264 tiles at most, which 256 places take one by one; a slot has
+    128 rows, as the 128 of the batch may be one sequence's, and a row 130 floats; beside them the shared ranges' rows."""
+    even, ragged = (ops.paged_attn_workspace_bytes(32, 32, 8, 128, 32, 2560, 2048, r) for r in (False, True))
+    rows = 32 * 32
+    assert ragged <= 264 * 128 * 130 * 4 + 32 * rows * 130 * 4 + rows * 8 + 64
