@@ -312,8 +312,8 @@ typedef struct q4_rope {
   float mscale;
 } q4_rope;
 
-/* y = x rotated at positions[t] (device int32, any sign), or with `inverse` rotated back (the transpose: the
- * gradient of x from that of y). x, y: T x heads x head_dim of dtype (F32, F16, BF16), rows and heads
+/* y = x rotated at positions[t] (device int32, any sign), or with `inverse` by the transpose (the gradient
+ * of x from that of y; the way back where mscale is 1). x, y: T x heads x head_dim of dtype (F32, F16, BF16), rows and heads
  * *_row and *_head elements apart (>= 0), the dims of a head next to each other. y may be x itself (same
  * strides); other overlaps are not allowed. Arithmetic in fp32, one rounding. head_dim even and <= 1024,
  * rot_dim even and <= head_dim, T * heads < 2^31, heads * head_dim < 2^27. T == 0 does nothing. */

@@ -7,8 +7,8 @@
 // read once per 16 to 128 rows instead of once per sequence. The keys of a sequence's own are a second kind of range.
 // Both run in one launch; a second joins the ranges of each row where there are several.
 //
-// Whole calls, back to back: one sequence of 700 keys (24/8 heads of 128, fp32) 9.7 us, a chain of dependent loads and two
-// launches; 32 sequences behind 2048 shared keys (32/8 heads, fp16) 21 us; 64 behind 16384 (24/8, fp32) 66 us.
+// Whole calls, back to back: one sequence of 700 keys (24/8 heads of 128, fp32) 9.9 us, a chain of dependent loads and two
+// launches; 32 sequences behind 2048 shared keys (32/8 heads, fp16) 21 us; 64 behind 16384 (24/8, fp32) 64 us.
 #include "q4_common.h"
 #include "q4_paged.h"
 
@@ -85,8 +85,8 @@ struct AttnArgs {
 // Rows (token, head of the group) of a workgroup where there are `rows` in all. Up to 16 rows are not enough to share the
 // keys among waves: each wave streams blocks of its own (paged_stream). Past them the waves share stages of keys
 // in LDS (paged_shared), 32 rows a wave: two waves for the rows and two for the keys, or four for the rows. 8 sequences of
-// 1000 to 6000 keys, 32/8 heads of 128, f16 (fp32): 4 rows in tiles of 16 and 64 31.9 and 34.8 us (32.3 and 37.2), 24
-// rows in tiles of 64 and 128 36.9 and 37.9 (39.4 and 44.3), 160 rows in tiles of 64 and 128 73 and 54 (81 and 75).
+// 1000 to 6000 keys, 32/8 heads of 128, f16 (fp32): 4 rows in tiles of 16 and 64 30.7 and 33.6 us (30.8 and 34.1), 24
+// rows in tiles of 64 and 128 35.6 and 37.3 (36.6 and 39.3), 160 rows in tiles of 64 and 128 73 and 61 (81 and 68).
 __host__ __device__ __forceinline__ int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : 128; }
 
 // The sequence of token t, another in each lane (batch or more: none). Every lane of the wave takes part.
@@ -119,15 +119,16 @@ constexpr int kMaxSplits = 64;  // ranges of a tile's keys
 
 // Ranges of each of `items` that share `places`: as many as fit at once, or, where those leave more than an eighth of the
 // places free, as many as fill them twice (the last ones start as the first end; `refill`: of many keys and few rows). One
-// token each of 12 / 20 / 24 sequences of 1000 to 6000 keys, 16 heads of 64: 49.7 / 79.9 / 86.3 -> 43.2 / 64.6 / 87.2 us;
-// 8 KV heads of 128, 24 / 40 sequences: 82 / 138 -> 74 / 115. Where they do fit (8 sequences of 16 heads), the second filling
-// costs: 33.5 -> 34.7 us; so it does for few keys (40 sequences of 1000 keys of 8 heads 27.8 -> 29.2, 2000 keys 45.6 -> 43.2)
-// and for more than 32 rows (80 of 2000 keys 59 -> 64).
+// token each of 12 / 20 / 24 sequences of 1000 to 6000 keys, 16 heads of 64: 46.9 / 74.4 / 79.6 -> 40.0 / 61.2 / 84.6 us;
+// 8 KV heads of 128, 24 / 40 sequences: 78 / 130 -> 70 / 109. Where they do fit (8 / 16 sequences of 16 heads), the second filling
+// costs: 31.6 / 53.4 -> 32.4 / 57.8 us; so it does for more than 32 rows (10 tokens each of 40 sequences of 2100 keys, 32/8 heads of
+// 128, 78 -> 84, of 80 with 16/4 of 64 43.4 -> 48.3). It gains as much below the limit of 2048 keys as above (40 sequences, 8
+// heads of 64: 2000 keys 47.0 -> 42.3, 2100 49.2 -> 44.2), and nothing at 1000.
 //
 // One each where the free places times the keys are few (no shared ranges, which need a join anyway): what splitting saves of the
 // time of an item, the free share of it, has to exceed what ranges cost, about that of 520 keys. 600 keys, 8 KV heads of 128,
-// 24 sequences of 1 / 30 / 100 tokens 19.2 / 35.2 / 65.9 -> 16.0 / 25.5 / 53 us; 2 of them 9.9 / 17.0 / 24.0 as they are, 11.9 /
-// 21.3 / 22.3 in one; 1000 keys, 8 and 24 of 100 tokens 38.4 / 90 -> 34.7 / 78.
+// 24 sequences of 1 / 30 / 100 tokens 18.5 / 33.5 / 67.5 -> 15.4 / 27.9 / 55.7 us; 2 of them 10.7 / 16.5 / 23.7 as they are, 11.4 /
+// 24.3 / 24.8 in one; 1000 keys, 8 and 24 of 100 tokens 42.7 / 95 -> 37.8 / 86.
 __host__ __device__ __forceinline__ int ranges_of(int items, int places, bool refill, int most, int keys) {
   if (places == kSlots && keys > 4 * kTurn && static_cast<int64_t>(places - items) * keys <= places * 520) return 1;
   int n = places / items;
@@ -352,8 +353,8 @@ constexpr float kGrow = CT == Q4_F16 ? 2.0f : 8.0f;
 
 // Eight softmax weights as the B operand of P V, in two terms of the cache's type that are multiplied one after the other: the weights
 // rounded, and what that leaves. One term alone put the results of fp16 and bf16 activations 1.35 times as far from the exact ones
-// as their own rounding does; two cost a third of the matrix products more (prompts behind 4096 shared keys 190 -> 239 us, 5 drafted tokens
-// each of 48 sequences 53 -> 61, single tokens up to 3%). The second term is formed while the first one's products run.
+// as their own rounding does; two cost half of the matrix products more (prompts behind 4096 shared keys 190 -> 239 us in replayed graphs,
+// 5 drafted tokens each of 48 sequences 53 -> 61, single tokens up to 3%). The second term is formed while the first one's products run.
 template <int CT>
 __device__ __forceinline__ vec8<CT> upper8(const float (&p)[8]) {
   typedef typename Num<CT>::type C2 __attribute__((ext_vector_type(2)));
@@ -405,7 +406,7 @@ __device__ __forceinline__ void store_o(const AttnArgs& a, const Item& it, const
 
 // Streaming form: 16 rows of one KV head, 32-key blocks dealt to the four waves, which keep (m, l, o) of their own and
 // join them at the end. What bounds it is the latency and bandwidth of the key loads: 8 sequences of 1000 to 6000 keys of 16
-// heads of 64 take 30 us, 3.8 TB/s (a large copy 5.1); two blocks a wave in flight instead of one spill or gain nothing.
+// heads of 64 take 32 us, 3.6 TB/s (a large copy 5.1); two blocks a wave in flight instead of one spill or gain nothing.
 //
 // Per block and wave: S^T = K Q^T (16x16x32 MFMA; K straight from memory to the A operand: lane r16 + 16 quad holds key
 // r16, dims 32 t + 8 quad ..), softmax per column (a lane holds 8 keys of one row, the other quads the rest), O^T +=
@@ -601,7 +602,8 @@ __device__ __forceinline__ void load_lds16(const unsigned char* src, unsigned ch
 // barrier a stage). With RW == 2 the two halves of the workgroup take the two 32-key blocks of a stage and join at the
 // end; with RW == 4 every wave takes both. What bounds it is the softmax between the two products of a block, which a wave
 // runs one after the other, and the two workgroups that the registers leave a compute unit: prompts of 8 sequences behind 4096
-// shared keys (32/8 heads of 128, bf16) take 185 us, 0.80 PFLOP/s (a large product 1.22), the matrix cores busy 36%.
+// shared keys (32/8 heads of 128, bf16) take 235 us, 0.63 PFLOP/s, or 0.95 with the weights' second term
+// (a large product 1.22), the matrix cores busy 44%.
 //
 // Per block and wave: S^T = K Q^T by 32x32x16 MFMA (lane: one row, half of the keys), softmax as above, O^T += V^T P^T with
 // the accumulators of S^T as the operand: lane half h supplies keys 16 u + 8 (i / 4) + 4 h + i % 4, and the transposing
@@ -879,7 +881,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(AttnArgs a) {
 }
 
 // Joins the ranges of each row: PG threads, each for every PG-th range, and those side by side for 4 dims of the row; the first
-// kB ranges of a thread are in flight at once. One launch and two dependent loads, 3 to 5 us, for a few rows; 6.8 us for the
+// kB ranges of a thread are in flight at once. One launch and two dependent loads, 4 to 5 us, for a few rows; 6.6 us for the
 // 20 MB of 7680 rows of 128 dims in four shared ranges and one own.
 template <int QT, int HD, int PG>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnArgs a) {
@@ -985,14 +987,15 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
   const int64_t rows = T * g;
   // The shared keys are a range of their own where that saves reading them once for each sequence: not for one sequence, not
   // for a few keys (they cost their ranges' partial results and join), and not where a sequence's rows alone fill tiles
-  // (prompts), which then read them as often either way and need no join. One token each of 2 / 8 / 32 sequences, 32/8
-  // heads of 128, 200 own keys, apart and not: 256 shared keys 9.1 / 12.9 / 16.1 and 9.0 / 10.4 / 15.0 us, 1024 keys
-  // 9.5 / 13.8 / 17.2 and 9.8 / 15.0 / 23.5, 16384 keys 20.7 / 27.2 / 36.1 and 26.5 / 54.5 / 163.
+  // (prompts), which then read them as often either way and join less. One token each of 2 / 8 / 32 sequences, 32/8
+  // heads of 128, 200 own keys, apart and not: 256 shared keys 9.2 / 11.6 / 15.8 and 10.1 / 10.0 / 12.2 us, 1024 keys
+  // 9.3 / 12.1 / 16.9 and 10.8 / 15.8 / 22.5, 16384 keys 19.0 / 22.3 / 34.3 and 25.1 / 49.5 / 158; 100 tokens each of 8 behind
+  // 4096 131 and 107.
   const bool apart = shared_len >= 4 * kTurn && batch > 1 && rows / batch < 128;
   p.own_from = apart ? shared_len : 0;
   if (apart) {
     // One workgroup for every compute unit: the other place of each is left to own ranges, and what ranges write and the join
-    // reads stays small (of 48 x 5 tokens x 32 heads and 4096 shared keys, 17 MB; with two 73 us, with one 62).
+    // reads stays small (of 48 x 5 tokens x 32 heads and 4096 shared keys, 17 MB; with two 70 us, with one 57).
     p.shared_tile = tile_rows(rows);
     const int64_t items = n_kv * static_cast<int64_t>(tiles_of(rows));
     p.shared_splits = static_cast<int>(std::max<int64_t>(
@@ -1007,8 +1010,8 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
     const int64_t items = static_cast<int64_t>(batch) * p.own_tiles * n_kv;
     // Short keys are one range, which needs no join: up to two blocks a wave always, up to four where there are items for a
     // quarter of the units. One token each of 1 / 4 / 12 / 32 sequences, 8 KV heads of 128, one range and as many as fit:
-    // 250 keys 7.8 / 7.9 / 8.9 / 10.5 and 8.8 / 8.8 / 10.6 / 13.6 us, 400 keys 9.9 / 10.0 / 11.4 / 14.1 and 8.9 / 10.0 /
-    // 12.5 / 16.9.
+    // 250 keys 7.9 / 8.1 / 8.6 / 10.2 and 10.1 / 10.1 / 10.7 / 13.3 us, 400 keys 9.7 / 10.2 / 11.0 / 13.6 and 10.2 / 10.2 /
+    // 12.8 / 16.9.
     const bool one = !apart && keys <= (items >= kSlots / 8 ? 4 : 2) * kTurn;
     p.own_most = one ? 1 : static_cast<int>(std::min<int64_t>((keys + kTurn - 1) / kTurn, kMaxSplits));
     if (ragged) {
@@ -1026,8 +1029,8 @@ Plan plan_for(int64_t T, int n_q, int n_kv, int batch, bool ragged, int L, int s
       p.slot_rows = tile_rows(rows / batch);
     }
     // One token each of 8 / 16 / 28 sequences of 1000 to 6000 keys, 16 heads of 64, the second ones longest first too and
-    // shortest first: 36.0 / 63.2 / 105 and 32.9 / 55.7 / 90 us. Up to three tokens each, 8 KV heads of 128, in the batch's order
-    // and so: 38.6 / 64.5 / 109 and 34.8 / 58.0 / 93.
+    // shortest first: 34.6 / 60.9 / 99 and 31.5 / 53.3 / 85 us. Up to three tokens each, 8 KV heads of 128, in the batch's order
+    // and so: 34.9 / 61.7 / 108 and 33.0 / 53.8 / 88.
     p.longest_first = batch > 1 && batch <= 64 && keys > 4 * kTurn;
     p.turn_from = INT32_MAX;
     if (!apart && !ragged && p.own_blocks <= kSlots) p.turn_from = (kSlots / 2 + n_kv * p.own_ranges - 1) / (n_kv * p.own_ranges);
@@ -1066,8 +1069,8 @@ int launch(const AttnArgs& a, int64_t blocks, int most, hipStream_t st) {
     hipLaunchKernelGGL((paged_attn_kernel<QT, CT, HD>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
   if (most > 1) {
     // (pg) a few ranges a thread, so that a row is one round trip; a thread a row where there are rows enough to fill the chip.
-    // With 1 / 4 / 8: one sequence of 700 keys 9.9 / 9.6 / 9.6 us, of 16000 30.8 / 21.8 / 20.3, 7680 rows of 5 ranges
-    // 57 / 58 / 61, 65000 rows of 2 to 4 ranges 191 / 204 / 218.
+    // With 1 / 4 / 8: one sequence of 700 keys 11.0 / 10.3 / 9.6 us, of 16000 29.5 / 20.8 / 19.4, 7680 rows of 5 ranges
+    // 57 / 57 / 59, 65000 rows of 2 to 4 ranges 234 / 244 / 257.
     const auto fn = pg == 1 ? paged_join_kernel<QT, HD, 1> : pg == 4 ? paged_join_kernel<QT, HD, 4> : paged_join_kernel<QT, HD, 8>;
     hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st, a);
   }

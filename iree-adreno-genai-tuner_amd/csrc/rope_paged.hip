@@ -143,7 +143,7 @@ __device__ __forceinline__ void fill_tables(float2* cs, const int* pos, int n, c
 }
 
 // x, y: T tokens of H heads; workgroup (x, y): tokens x * tpb .., part y of their units. HBM bound: 8192 tokens of 40 heads of
-// 128 dims in bf16 29.8 us, 5.6 TB/s; 8 tokens of 32 heads 2.9 us, the launch and two dependent loads.
+// 128 dims in bf16 30.1 us, 5.6 TB/s; 8 tokens of 32 heads 3.0 us, the launch and two dependent loads.
 template <int DT, int LAYOUT, int VB, bool NT>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const void* x_, int64_t xr, int64_t xh, void* y_, int64_t yr,
                                                        int64_t yh, int T, int tpb, int H, int units, int part,
@@ -211,7 +211,7 @@ __device__ __forceinline__ int sequence_of(const PagedBatch& b, int t) {
 }
 
 // The same over the heads of k, v and q of each token, with the row of the cache looked up beside the tables. HBM bound: prompts
-// of 16 sequences (8000 tokens, 32/8 heads of 128 in bf16) 39.7 us, 5.1 TB/s; 32 tokens 4.2 us, three dependent loads.
+// of 16 sequences (8000 tokens, 32/8 heads of 128 in bf16) 40.1 us, 5.0 TB/s; 32 tokens 4.2 us, three dependent loads.
 template <int DT, int CT, int LAYOUT, int VB, bool NT>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
   typedef Unit<DT, LAYOUT, VB> U;
@@ -380,7 +380,7 @@ int launch_append1(int vb, int layout, AppendArgs& a, hipStream_t st) {
 
 // The widest vectors, in bytes, in which heads of hd dims with `half` rotated pairs, operands at these addresses and these
 // strides are whole (the interleaved layout needs no boundary between its rotated pairs and the rest on a vector);
-// 0: none. Odd halves and starts go element by element (8192 tokens of 40 heads, 62 of 128 dims rotated by halves: 74 us).
+// 0: none. Odd halves and starts go element by element (8192 tokens of 40 heads, 62 of 128 dims rotated by halves: 70 us).
 int vector_bytes(int hd, int half, int layout, size_t es, std::initializer_list<const void*> at,
                  std::initializer_list<int64_t> strides) {
   for (const int vb : {16, 8}) {

@@ -8,8 +8,8 @@
 // Two launches, each one pass: the first decides j (every wave for itself: two dependent round trips instead of a
 // launch) and sums w over chunks of kChunk values, a wave each; the second finds the chunk by a scan of the chunk sums, and
 // reads that chunk again for the index. Only one row of p and one of q is read in full, whatever the number
-// of drafts. Bound: HBM for large batches (64 rows of 128256 values 19.4 us, 3.4 TB/s: the sums 15.9, the pick 4.6), the
-// dependent loads and two launches for one sequence (32000 values 8.1 us).
+// of drafts. Bound: HBM for large batches (64 rows of 128256 values 19.8 us, 3.3 TB/s: the sums 15.6, the pick 4.6; 13.9 without
+// draft_probs), the dependent loads and two launches for one sequence (32000 values 9.5 us).
 #include "q4_common.h"
 
 #include <algorithm>

@@ -504,7 +504,7 @@ def _paged_c(k_cache, v_cache, page_table, seq_lens, cu_q, dtype, tokens, n_kv=N
 
 def rope_rotate(x, positions, rope, inverse=False, out=None):
     """x [T, heads, hd] (fp32, fp16 or bf16, rows and heads may be strided) rotated at positions [T] (device int32) by
-    `rope` (q4llm.rope.Rope); `inverse` rotates back (the gradient). `out` may be x."""
+    `rope` (q4llm.rope.Rope); `inverse`: the transpose, which is the gradient, and rotates back where mscale is 1. `out` may be x."""
     y = _rope(x, positions, *rope, inverse, out)
     if y is not None:
         return y
