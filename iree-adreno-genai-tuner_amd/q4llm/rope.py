@@ -71,7 +71,7 @@ def rope_tables(cfg: dict, max_ctx: int):
 # The keys of a config's scaling that rope_params goes by (some have no effect on a type and are often there all the same).
 _ROPE_KEYS = {"rope_type", "type", "rope_theta", "factor", "original_max_position_embeddings", "partial_rotary_factor"}
 _SCALING_KEYS = {"default": set(), "linear": set(), "dynamic": set(), "llama3": {"low_freq_factor", "high_freq_factor"},
-                 "yarn": {"beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"}}
+                 "yarn": {"beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate", "finetuned"}}
 
 
 def rope_params(cfg: dict, seq_len: int = None, interleaved: bool = False) -> Rope:

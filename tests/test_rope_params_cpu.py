@@ -64,8 +64,9 @@ def test_unknown_keys_are_refused(scaling):
 
 
 def test_keys_without_a_value_are_none():
+    """(And `finetuned`, which tells only how a model was made.)"""
     a = rope_params({**CFG, "rope_scaling": {"rope_type": "yarn", "factor": 4.0}})
-    b = rope_params({**CFG, "rope_scaling": {"type": "yarn", "rope_type": "yarn", "factor": 4.0, "mscale": None, "attention_factor": None,
+    b = rope_params({**CFG, "rope_scaling": {"type": "yarn", "rope_type": "yarn", "factor": 4.0, "mscale": None, "attention_factor": None, "finetuned": True,
                                              "short_factor": None}})
     assert torch.equal(a.inv_freq, b.inv_freq) and a.mscale == b.mscale
 
