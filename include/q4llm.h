@@ -323,7 +323,7 @@ int rope_rotate(const void* x, int64_t x_row, int64_t x_head, void* y, int64_t y
 
 /* A paged KV cache and the batch that one step runs on it. k_cache, v_cache: [num_pages, page_size, n_kv,
  * head_dim] of dtype F16 or BF16, num_pages * page_size < 2^31. Key j of sequence b is row j % page_size of
- * page page_table[b * table_stride + j / page_size] (device int32; entries outside [0, num_pages) hold no
+ * page page_table[b * table_stride + j / page_size] (device int32, table_stride >= max_pages; entries outside [0, num_pages) hold no
  * key; positions from max_pages * page_size on have no page). seq_lens: device int32 [batch], the keys of
  * each sequence, those of this step's tokens included. The T tokens of a step lie sequence after sequence:
  * cu_q (device int32 [batch + 1], ascending from 0) gives each sequence's first, tokens from cu_q[batch] on

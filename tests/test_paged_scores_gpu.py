@@ -92,3 +92,26 @@ def test_one_key_far_above_the_others(dev, dt, rows, g, above):
     line = Line(dev, dt, scores, v, 64, rows, g)
     # as above; and with an fp16 cache a weight is off by 2^-25, half of fp16's smallest step, where the largest one is 2^12 or more
     line.check((2 * line.most * 2.0 ** -22 + 2 * weight_step(dt) + (n + 40) * U, 0.0 if dt == torch.bfloat16 else n * 2.0 ** -37))
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows,g", FORMS, ids=FORM_IDS)
+def test_scores_near_the_limit_of_fp16_caches(dev, dt, rows, g):
+    """Scores up to 9 million, where those of two keys are equal or thousands apart: the values of the highest ones."""
+    n, n_kv, hd = 700, 16, 64
+    gen = torch.Generator().manual_seed(7 * rows)
+    ct = torch.bfloat16 if dt == torch.bfloat16 else torch.float16
+    scores = ((torch.rand(n, generator=gen) * 2 - 1) * 60000).to(ct).float()
+    line = Line(dev, dt, scores, torch.randn(n, n_kv, hd, generator=gen), 32, rows, g)
+    line.q *= 150
+    s, w = scores.double(), line.v.cpu()  # (of the pages: the reference is built from the same values as Line's)
+    assert w.isfinite().all() and s.abs().max() * 150 < 1e7
+    seen = torch.arange(n)[None] <= torch.arange(n - rows, n)[:, None]
+    top = torch.where(seen, s, float("-inf"))
+    top = (top == top.amax(-1, keepdim=True)).double()
+    p = top / top.sum(-1, keepdim=True)
+    order = torch.randperm(-(-n // 16), generator=torch.Generator().manual_seed(n))
+    v = w[order].flatten(0, 1)[:n].double()
+    line.ref, line.size = (torch.einsum("rn,nhd->rhd", p, x) for x in (v, v.abs()))
+    # equal scores have equal weights, and all others none: the sums of at most n equal weights, and the quotient
+    line.check((2 * weight_step(dt) + (n + 40) * U, 0.0))
